@@ -1,0 +1,483 @@
+// attention.hip -- softmax(scale q k^T + mask) v over 4-D views [batch, heads, sequence, head dim], with causal masks,
+// sliding windows, leading keys that stay visible, shared key heads and a length per sequence, in one pass over the keys:
+// running maximum m and sum l per query, out = sum_j exp(x_j - m) v_j / l, lse = m + log l.
+//
+//   attention_k        many queries: 128 queries of one head per workgroup, tiles of 64 keys through LDS;
+//   attention_split_k  few queries (single tokens over a cache): the queries of all heads that share a key head are the
+//                      rows of one 16-row tile, waves and workgroups split the keys, attention_join_k adds them up.
+#pragma clang fp contract(fast)
+
+#include "attention.hpp"
+#include "attention_host.hpp"
+
+using namespace aixd;
+using namespace aixk;
+using namespace aixk::attn;
+
+namespace {
+
+struct ForwardArgs {
+    Shape s;
+    View q, k, v, out;
+    float* lse;
+    u32 tiles;                                // 128-row tiles per head
+    i32 whole;                                // results in 4-element groups
+};
+
+// Scores are formed transposed, S^T = K Q^T with v_mfma 32x32: a lane then holds 16 of 32 keys of ONE query (lane % 32), the
+// row statistics are lane-local but for one exchange between the halves of the wave, and the accumulators, rounded, are
+// the second operand of O^T = V^T P^T as they lie -- the transposed reads of V number the keys the same way.  The running
+// maximum is only raised when some query of the wave passes it by a factor 2^8 (exact either way: any reference that
+// keeps exp in range gives the same quotient), so the accumulators are rarely rescaled.  P is rounded to the operands'
+// type for the second product, as the matrix unit takes it; the sum is taken from the f32 values.
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attention_k(ForwardArgs a)
+{
+    typedef Mma<T> M;
+    typedef typename M::Frag Frag;
+    typedef Tile<T, DP> L;
+    constexpr int KT = 64, DB = DP / 32, DC = DP / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char* ks = lds;
+    char* vs = lds + KT * L::PITCH;
+    const Shape& s = a.s;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    const u32 id = xcd_order(blockIdx.x, gridDim.x);
+    const u32 head = id / a.tiles, tile = a.tiles - 1 - id % a.tiles;       // longest rows of a causal mask first
+    const u32 b = head / s.H, h = head % s.H, hk = h / s.G;
+    const Row r = row_of(s, b);
+    const T* K = (const T*)a.k.p + b * a.k.b + hk * a.k.h;
+    const T* V = (const T*)a.v.p + b * a.v.b + hk * a.v.h;
+
+    const i32 i0 = (i32)tile * 128, i1 = i0 + 127 < s.SQ ? i0 + 127 : s.SQ - 1;
+    const i32 w0 = i0 + wave * 32, w1 = w0 + 31 < s.SQ ? w0 + 31 : s.SQ - 1;      // this wave's queries (w0 > w1: none)
+    const i32 i = w0 + (lane & 31);
+    const i32 p = r.start + i;
+    const bool on = i < s.SQ;
+
+    Frag q[DC];
+    {
+        const T* row = (const T*)a.q.p + b * a.q.b + h * a.q.h + (u64)(on ? i : 0) * a.q.s;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) q[c] = load8<T>(row, c * 16 + half * 8, s.DW, on);
+    }
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x16{};
+    float m = -__builtin_inff(), l = 0.0f;                    // m in units of log2, l this half's part of the sum
+    const float c2 = s.scale * kLog2e;
+
+    const Tiles t = tiles_of(s, r.length, r.start + i0, r.start + i1, KT);
+    Stage<T, DP, KT, 256> sk, sv;
+    if (t.n) {
+        const i32 j0 = tile_at(t, 0) * KT;
+        sk.load(K, a.k.s, j0, r.length, s.DW, tid);
+        sv.load(V, a.v.s, j0, r.length, s.DW, tid);
+    }
+    for (i32 n = 0; n < t.n; ++n) {
+        const i32 j0 = tile_at(t, n) * KT;
+        __syncthreads();
+        sk.store(ks, j0, r.length, s.DW, tid);
+        sv.store(vs, j0, r.length, s.DW, tid);
+        __syncthreads();
+        if (n + 1 < t.n) {
+            const i32 next = tile_at(t, n + 1) * KT;
+            sk.load(K, a.k.s, next, r.length, s.DW, tid);
+            sv.load(V, a.v.s, next, r.length, s.DW, tid);
+        }
+        if (w0 > w1 || none_visible(s, r.length, r.start + w0, r.start + w1, j0, j0 + KT - 1)) continue;
+
+        f32x16 x[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            x[kb] = f32x16{};
+#pragma unroll
+            for (int c = 0; c < DC; ++c) x[kb] = M::run32(L::row(ks, kb * 32 + (lane & 31), 2 * c + half), q[c], x[kb]);
+        }
+        if (!all_visible(s, r.length, r.start + w0, r.start + w1, j0, j0 + KT - 1)) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const i32 j = j0 + kb * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
+                    x[kb][v] = visible(s, r.length, p, j) ? x[kb][v] : -__builtin_inff();
+                }
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) top = fmaxf(top, x[kb][v]);
+        top = fmaxf(top, other_half(top)) * c2;
+        if (__any(top > m + 8.0f)) {                          // (m = -inf: any visible key)
+            const float raised = fmaxf(m, top);
+            const float keep = raised == -__builtin_inff() ? 0.0f : exp2_of(m - raised);
+            m = raised;
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[d][v] *= keep;
+        }
+        const float ref = m == -__builtin_inff() ? 0.0f : m;   // a row without a visible key so far: every term is exp(-inf)
+        Frag w[4];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            float e[16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) { e[v] = exp2_of(x[kb][v] * c2 - ref); l += e[v]; }
+            w[2 * kb] = M::pack8(e);
+            w[2 * kb + 1] = M::pack8(e + 8);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] = M::run32(L::column(vs, c * 16, d, lane), w[c], o[d]);
+    }
+
+    l += other_half(l);
+    if (!on) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;            // a row that sees nothing: zeros
+    if (a.lse && half == 0) a.lse[((u64)b * s.H + h) * (u64)s.SQ + (u32)i] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * kLn2;
+    char* row = a.out.p + (b * a.out.b + h * a.out.h + (u64)(u32)i * a.out.s) * sizeof(T);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            put4<T>(row, a.out.d, a.whole, d * 32 + g * 8 + half * 4, s.D, o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
+}
+
+// ---- few queries ----------------------------------------------------------------------------------------------------------
+
+struct SplitArgs {
+    Shape s;
+    View q, k, v, out;
+    float* lse;
+    u32 tiles, splits;                        // 16-row tiles per key head, shares of the keys
+    i32 whole;
+    float* part_o;                            // [split][batch * heads * queries][DP]
+    float* part_ml;                           // [split][batch * heads * queries][2]: maximum (log2), sum
+};
+
+constexpr int kSplitWaves = 4, kSplitKeys = 32;        // keys per wave and step
+
+template <class T, int DP> struct SplitLds {
+    static constexpr int kSlab = kSplitKeys * DP * (int)sizeof(T);                        // a wave's keys of V
+    static constexpr int kJoin = kSplitWaves * (16 * DP + 32) * 4;                           // accumulators, maxima and sums of all waves
+    static constexpr int kBytes = kSlab * kSplitWaves > kJoin ? kSlab * kSplitWaves : kJoin;
+};
+
+// Row r of a key head's R = G * SQ rows is query r % SQ of head r / SQ of the group.  16 rows against 32 keys with v_mfma
+// 16x16: keys are read from memory straight as the first operand; V goes through a slab of LDS that belongs to the wave
+// alone (no barrier in the loop) to be read transposed.  Reading the cache is the bound, so the next step's words are in
+// flight while a step is computed.
+template <class T, int DP>
+__global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs a)
+{
+    typedef Mma<T> M;
+    typedef typename M::Frag Frag;
+    constexpr int KT = kSplitKeys, DC = DP / 32, DB = DP / 16, WORDS = DP * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T), PITCH = DP * (int)sizeof(T);
+    constexpr int NV = KT * WORDS / 64;                        // 16-byte words of V per lane
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const Shape& s = a.s;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c15 = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    char* slab = lds + wave * SplitLds<T, DP>::kSlab;
+
+    const u32 id = blockIdx.x, split = id % a.splits, rest = id / a.splits;
+    const u32 tile = rest % a.tiles, bk = rest / a.tiles, b = bk / s.HK, hk = bk % s.HK;
+    const Row r = row_of(s, b);
+    const u32 R = s.G * (u32)s.SQ, r0 = tile * 16, r1 = r0 + 15 < R ? r0 + 15 : R - 1;
+    const u32 rr = r0 + c15;
+    const bool on = rr < R;
+    const i32 i = (i32)((on ? rr : 0) % (u32)s.SQ), p = r.start + i;
+    const u32 h = hk * s.G + (on ? rr : 0) / (u32)s.SQ;
+    const bool one_head = r0 / (u32)s.SQ == r1 / (u32)s.SQ;
+    const i32 p0 = r.start + (one_head ? (i32)(r0 % (u32)s.SQ) : 0), p1 = r.start + (one_head ? (i32)(r1 % (u32)s.SQ) : s.SQ - 1);
+
+    Frag q[DC];
+    {
+        const T* row = (const T*)a.q.p + b * a.q.b + h * a.q.h + (u64)(u32)i * a.q.s;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) q[c] = load8<T>(row, c * 32 + g * 8, s.DW, on);
+    }
+    const T* K = (const T*)a.k.p + b * a.k.b + hk * a.k.h;
+    const T* V = (const T*)a.v.p + b * a.v.b + hk * a.v.h;
+    f32x4 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x4{};
+    float m = -__builtin_inff(), l = 0.0f;
+    const float c2 = s.scale * kLog2e;
+
+    // this workgroup's share of the visible steps; its waves take them in turn
+    const Tiles t = tiles_of(s, r.length, p0, p1, KT);
+    const i32 from = (i32)((u64)(u32)t.n * split / a.splits), to = (i32)((u64)(u32)t.n * (split + 1) / a.splits);
+
+    // slot of 16-byte word c of key k in the slab: the transposed reads take 32 bytes from each of eight keys at a time
+    auto turn = [](int k) { return WORDS >= 16 ? ((k & 7) << 1) | ((k >> 3) & 1) : ((k >> 1) & 3) << 1; };
+    const int last = (int)s.DW / PER - 1;
+    Frag kf[2][DC];
+    u32x4 vf[NV];
+    auto load = [&](i32 j0) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const i32 j = j0 + kb * 16 + c15;
+            const T* row = K + (u64)(u32)(j < r.length ? j : r.length - 1) * a.k.s;
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                if constexpr (sizeof(T) == 2) { const int w = c * 4 + g; kf[kb][c] = *(const u32x4*)(row + (w < last ? w : last) * 8); }
+                else {
+                    const int w = c * 8 + g * 2;
+                    kf[kb][c].lo = *(const f32x4*)(row + (w < last ? w : last) * 4);
+                    kf[kb][c].hi = *(const f32x4*)(row + (w + 1 < last ? w + 1 : last) * 4);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int e = lane + n * 64, w = e % WORDS;
+            const i32 j = j0 + e / WORDS;
+            vf[n] = *(const u32x4*)(V + (u64)(u32)(j < r.length ? j : r.length - 1) * a.v.s + (w < last ? w : last) * PER);
+        }
+    };
+    i32 n = from + wave;
+    if (n < to) load(tile_at(t, n) * KT);
+    for (; n < to; n += kSplitWaves) {
+        const i32 j0 = tile_at(t, n) * KT;
+        f32x4 x[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            x[kb] = f32x4{};
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                // (words past the head dim repeat the last one: the query's zeros would meet an infinity there as a NaN)
+                Frag f = kf[kb][c];
+                if constexpr (sizeof(T) == 2) { if (c * 32 + g * 8 >= (int)s.DW) f = M::zero(); }
+                else { if (c * 32 + g * 8 >= (int)s.DW) f.lo = f32x4{}; if (c * 32 + g * 8 + 4 >= (int)s.DW) f.hi = f32x4{}; }
+                x[kb] = M::run16(f, q[c], x[kb]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < NV; ++e) {
+            const int at = lane + e * 64, k = at / WORDS, w = at % WORDS;
+            *(u32x4*)(slab + k * PITCH + ((w ^ turn(k)) << 4)) = j0 + k < r.length && w <= last ? vf[e] : u32x4{0, 0, 0, 0};
+        }
+        if (n + kSplitWaves < to) load(tile_at(t, n + kSplitWaves) * KT);
+
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                x[kb][v] = visible(s, r.length, p, j0 + kb * 16 + 4 * g + v) ? x[kb][v] * c2 : -__builtin_inff();
+                top = fmaxf(top, x[kb][v]);
+            }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (__any(top > m + 8.0f)) {
+            const float raised = fmaxf(m, top);
+            const float keep = raised == -__builtin_inff() ? 0.0f : exp2_of(m - raised);
+            m = raised;
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) o[d][v] *= keep;
+        }
+        const float ref = m == -__builtin_inff() ? 0.0f : m;
+        float e[8];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) { e[4 * kb + v] = exp2_of(x[kb][v] - ref); l += e[4 * kb + v]; }
+        const Frag w = M::pack8(e);
+        // column 16 d + lane % 16 of V, the keys 16 (j / 4) + 4 g + j % 4 of element j
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            Frag f;
+            if constexpr (sizeof(T) == 2) {
+                const int k = 4 * g + (c15 >> 2), word = 2 * d + ((c15 & 3) >> 1);
+                const char* lo = slab + k * PITCH + ((word ^ turn(k)) << 4) + 8 * (c15 & 1);
+                const char* hi = slab + (k + 16) * PITCH + ((word ^ turn(k + 16)) << 4) + 8 * (c15 & 1);
+                const u32x2 lw = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lo));
+                const u32x2 hw = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi));
+                f = u32x4{lw.x, lw.y, hw.x, hw.y};
+            } else {
+                float y[8];
+                const int c = 16 * d + c15;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { const int k = 16 * (j >> 2) + 4 * g + (j & 3); y[j] = *(const float*)(slab + k * PITCH + (((c >> 2) ^ turn(k)) << 4) + 4 * (c & 3)); }
+                f = M::pack8(y);
+            }
+            o[d] = M::run16(f, w, o[d]);
+        }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+
+    // the waves' shares: [wave][16 rows][DP] accumulators, then maxima and sums
+    __syncthreads();
+    float* all = (float*)lds;
+    float* ml = all + kSplitWaves * 16 * DP;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) *(f32x4*)(all + (wave * 16 + c15) * DP + ((d * 16 + 4 * g) ^ (4 * (c15 & 7)))) = o[d];
+    if (g == 0) { ml[(wave * 16 + c15) * 2] = m; ml[(wave * 16 + c15) * 2 + 1] = l; }
+    __syncthreads();
+    const u64 rows = (u64)s.B * s.H * (u32)s.SQ;
+    for (int e = tid; e < 16 * DP / 4; e += kSplitWaves * 64) {
+        const int row = e / (DP / 4), d = e % (DP / 4) * 4;
+        if (r0 + row >= R) continue;
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < kSplitWaves; ++w) top = fmaxf(top, ml[(w * 16 + row) * 2]);
+        f32x4 sum = f32x4{};
+        float total = 0.0f;
+        if (top != -__builtin_inff()) {
+#pragma unroll
+            for (int w = 0; w < kSplitWaves; ++w) {
+                const float f = exp2_of(ml[(w * 16 + row) * 2] - top);
+                total += f * ml[(w * 16 + row) * 2 + 1];
+                sum += f * *(const f32x4*)(all + (w * 16 + row) * DP + (d ^ (4 * (row & 7))));
+            }
+        }
+        const u32 qi = (r0 + row) % (u32)s.SQ, qh = hk * s.G + (r0 + row) / (u32)s.SQ;
+        const u64 at = ((u64)b * s.H + qh) * (u32)s.SQ + qi;
+        if (a.splits > 1) {
+            *(f32x4*)(a.part_o + (split * rows + at) * DP + d) = sum;
+            if (d == 0) *(f32x2*)(a.part_ml + (split * rows + at) * 2) = f32x2{top, total};
+        } else {
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            if (a.lse && d == 0) a.lse[at] = total == 0.0f ? -__builtin_inff() : (top + log2f(total)) * kLn2;
+            put4<T>(a.out.p + (b * a.out.b + qh * a.out.h + (u64)qi * a.out.s) * sizeof(T), a.out.d, a.whole, d, s.D, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+        }
+    }
+}
+
+// the shares of the keys added up in their order: 64 lanes on DP / 4 groups of four, four rows per workgroup
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attention_join_k(SplitArgs a)
+{
+    constexpr int LANES = DP / 4;                              // lanes per row
+    const Shape& s = a.s;
+    const u64 rows = (u64)s.B * s.H * (u32)s.SQ;
+    const u64 at = (u64)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const u32 d = threadIdx.x % LANES * 4;
+    if (at >= rows) return;
+    float top = -__builtin_inff();
+    for (u32 k = 0; k < a.splits; ++k) top = fmaxf(top, a.part_ml[(k * rows + at) * 2]);
+    f32x4 sum = f32x4{};
+    float total = 0.0f;
+    if (top != -__builtin_inff()) {
+        for (u32 k = 0; k < a.splits; ++k) {
+            const f32x2 ml = *(const f32x2*)(a.part_ml + (k * rows + at) * 2);
+            const float f = exp2_of(ml.x - top);
+            total += f * ml.y;
+            sum += f * *(const f32x4*)(a.part_o + (k * rows + at) * DP + d);
+        }
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    if (a.lse && d == 0) a.lse[at] = total == 0.0f ? -__builtin_inff() : (top + log2f(total)) * kLn2;
+    const u32 i = (u32)(at % (u32)s.SQ), h = (u32)(at / (u32)s.SQ % s.H), b = (u32)(at / (u32)s.SQ / s.H);
+    put4<T>(a.out.p + (b * a.out.b + h * a.out.h + (u64)i * a.out.s) * sizeof(T), a.out.d, a.whole, d, s.D, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+}
+
+// ---- operands the kernels cannot read where they lie ----------------------------------------------------------------------
+// [batch, heads, sequence, D] through any strides into dense rows of DW elements (whole 16-byte words), zeros behind D.
+template <class T>
+__global__ __launch_bounds__(256) void attention_pack_k(View src, T* dst, u32 H, u64 S, u32 D, u32 DW, u64 total)
+{
+    for (u64 e = (u64)blockIdx.x * 256 + threadIdx.x; e < total; e += (u64)gridDim.x * 256) {
+        const u32 d = (u32)(e % DW);
+        const u64 row = e / DW, i = row % S, bh = row / S, h = bh % H, b = bh / H;
+        dst[e] = d < D ? ((const T*)src.p)[b * src.b + h * src.h + i * src.s + d * src.d] : zero<T>();
+    }
+}
+
+} // namespace
+
+namespace aixk {
+namespace attn {
+
+int pack(aixk_ctx* ctx, int dtype, const View& src, void* dst, u32 B, u32 H, u64 S, u32 D, u32 DW)
+{
+    const u64 total = (u64)B * H * S * DW;
+    if (!total) return AIXK_OK;
+    const unsigned blocks = grid_for(total, 256, (unsigned)ctx->cus * 16u);
+    if (dtype == AIXK_F32) hipLaunchKernelGGL((attention_pack_k<float>), dim3(blocks), dim3(256), 0, ctx->stream, src, (float*)dst, H, S, D, DW, total);
+    else if (dtype == AIXK_F16) hipLaunchKernelGGL((attention_pack_k<f16>), dim3(blocks), dim3(256), 0, ctx->stream, src, (f16*)dst, H, S, D, DW, total);
+    else hipLaunchKernelGGL((attention_pack_k<bf16>), dim3(blocks), dim3(256), 0, ctx->stream, src, (bf16*)dst, H, S, D, DW, total);
+    AIXK_HIP(hipGetLastError());
+    return AIXK_OK;
+}
+
+namespace {
+
+template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
+{
+    const Shape& s = c.s;
+    const u64 rows = (u64)s.B * s.H * (u32)s.SQ;
+    const u32 R = s.G * (u32)s.SQ;
+    const u64 wide = (u64)s.B * s.H * (((u32)s.SQ + 127) / 128), narrow = (u64)s.B * s.HK * ((R + 15) / 16);
+    // Few queries: at most 32 rows per key head.
+    if (R > 32) {
+        AIXK_REQUIRE(wide < (1ull << 31), "attention: too many rows");
+        ForwardArgs a{s, c.q, c.k, c.v, c.out, c.lse, ((u32)s.SQ + 127) / 128, c.whole_out};
+        constexpr size_t lds = 2 * 64 * DP * sizeof(T);
+        AIXK_TRY(allow_lds(attention_k<T, DP>, lds));
+        hipLaunchKernelGGL((attention_k<T, DP>), dim3((unsigned)wide), dim3(256), lds, ctx->stream, a);
+        AIXK_HIP(hipGetLastError());
+        return AIXK_OK;
+    }
+    SplitArgs a{s, c.q, c.k, c.v, c.out, c.lse, (R + 15) / 16, 1, c.whole_out, nullptr, nullptr};
+    // Shares of the keys until every compute unit has four workgroups, but no share below one step of all waves.  What a row
+    // can see at most bounds the steps: the whole cache, or the window and the leading keys.
+    u64 keys = (u64)s.SK;
+    if (s.window && (u64)s.window + (u64)s.SQ + (u64)s.sinks < keys) keys = (u64)s.window + (u64)s.SQ + (u64)s.sinks;
+    const u64 steps = (keys + kSplitKeys * kSplitWaves - 1) / (kSplitKeys * kSplitWaves);
+    u64 splits = ((u64)ctx->cus * 4 + narrow - 1) / narrow;
+    if (splits > steps) splits = steps;
+    if (splits < 1) splits = 1;
+    AIXK_REQUIRE(narrow * splits < (1ull << 31), "attention: too many rows");
+    a.splits = (u32)splits;
+    if (splits > 1) {
+        const size_t o_bytes = (size_t)splits * rows * DP * sizeof(float);
+        void* ws;
+        AIXK_TRY(block_scratch(ctx, kScratchParts, o_bytes + (size_t)splits * rows * 2 * sizeof(float), &ws));
+        a.part_o = (float*)ws;
+        a.part_ml = (float*)((char*)ws + o_bytes);
+    }
+    constexpr size_t lds = SplitLds<T, DP>::kBytes;
+    AIXK_TRY(allow_lds(attention_split_k<T, DP>, lds));
+    hipLaunchKernelGGL((attention_split_k<T, DP>), dim3((unsigned)(narrow * splits)), dim3(kSplitWaves * 64), lds, ctx->stream, a);
+    AIXK_HIP(hipGetLastError());
+    if (splits > 1) {
+        constexpr u32 per = 256 / (DP / 4);
+        hipLaunchKernelGGL((attention_join_k<T, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, ctx->stream, a);
+        AIXK_HIP(hipGetLastError());
+    }
+    return AIXK_OK;
+}
+
+} // namespace
+} // namespace attn
+} // namespace aixk
+
+extern "C" int32_t aixk_attention(aixk_ctx* ctx, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* v, const aixk_attention_spec* spec,
+                                  const aixhip_tensor* out, const aixhip_tensor* lse)
+{
+    Call c;
+    AIXK_TRY(c.shape("attention", q, k, v, spec));
+    AIXK_TRY(c.result("attention", out, q, "the result", &c.out, &c.whole_out));
+    if (lse) AIXK_TRY(c.statistics("attention", lse, q, &c.lse));
+    const aixhip_tensor* inputs[] = {q, k, v, spec->lengths, spec->starts};
+    for (const aixhip_tensor* in : inputs) AIXK_REQUIRE(!overlap(out, in) && !overlap(lse, in), "attention: a result overlaps an operand");
+    AIXK_REQUIRE(!overlap(out, lse), "attention: the results overlap");
+    AIXK_TRY(set_device(ctx));
+    if (c.s.B == 0 || c.s.H == 0 || c.s.SQ == 0) return AIXK_OK;
+    AIXK_TRY(c.operand(ctx, q, kScratchQ, &c.q));
+    AIXK_TRY(c.operand(ctx, k, kScratchK, &c.k));
+    AIXK_TRY(c.operand(ctx, v, kScratchV, &c.v));
+    return c.by_type([&](auto type, auto width) { return forward<decltype(type), decltype(width)::value>(ctx, c); });
+}

@@ -1,0 +1,374 @@
+// attention_backward.hip -- the gradients of attention.hip's softmax(scale q k^T + mask) v from the saved lse:
+//     P = exp(scale q k^T - lse)     delta = sum_d grad out     dS = P (grad v^T - delta)
+//     dq = scale dS k                dk = scale dS^T q          dv = P^T grad
+// in two passes without atomics: attention_dq_k walks the keys for a block of queries (and leaves delta for the other),
+// attention_dkdv_k walks the queries of all heads that share a block of keys.  Each forms the scores again; seven products
+// instead of the five of a single pass that would add dq with atomics in an order of their own.
+#pragma clang fp contract(fast)
+
+#include "attention.hpp"
+#include "attention_host.hpp"
+
+using namespace aixd;
+using namespace aixk;
+using namespace aixk::attn;
+
+namespace {
+
+struct BackwardArgs {
+    Shape s;
+    View grad, q, k, v, y, dq, dk, dv;
+    const float* lse;
+    float* delta;
+    u32 tiles;                                // row tiles per head (dq), key tiles per key head (dk, dv)
+    u32 splits;                               // shares of the queries (dk, dv)
+    i32 whole_dq, whole_dk, whole_dv;
+    float* part;                              // [split][dk, dv][batch * key heads * keys][DP]
+};
+
+// As in attention_k the scores are transposed (a lane = one query): dS^T, rounded, feeds dq^T = K^T dS^T as it lies.
+template <class T, int DP, int KT>
+__global__ __launch_bounds__(256) void attention_dq_k(BackwardArgs a)
+{
+    typedef Mma<T> M;
+    typedef typename M::Frag Frag;
+    typedef Tile<T, DP> L;
+    constexpr int DB = DP / 32, DC = DP / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char* ks = lds;
+    char* vs = lds + KT * L::PITCH;
+    const Shape& s = a.s;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    const u32 id = xcd_order(blockIdx.x, gridDim.x);
+    const u32 head = id / a.tiles, tile = a.tiles - 1 - id % a.tiles;
+    const u32 b = head / s.H, h = head % s.H, hk = h / s.G;
+    const Row r = row_of(s, b);
+    const T* K = (const T*)a.k.p + b * a.k.b + hk * a.k.h;
+    const T* V = (const T*)a.v.p + b * a.v.b + hk * a.v.h;
+    const i32 i0 = (i32)tile * 128, i1 = i0 + 127 < s.SQ ? i0 + 127 : s.SQ - 1;
+    const i32 w0 = i0 + wave * 32, w1 = w0 + 31 < s.SQ ? w0 + 31 : s.SQ - 1;
+    const i32 i = w0 + (lane & 31), p = r.start + i;
+    const bool on = i < s.SQ;
+    const u64 at = ((u64)b * s.H + h) * (u64)(u32)s.SQ + (u32)i;
+
+    Frag q[DC], go[DC];
+    float delta = 0.0f;
+    {
+        const u64 row = (u64)(u32)(on ? i : 0);
+        const T* rq = (const T*)a.q.p + b * a.q.b + h * a.q.h + row * a.q.s;
+        const T* rg = (const T*)a.grad.p + b * a.grad.b + h * a.grad.h + row * a.grad.s;
+        const T* ry = (const T*)a.y.p + b * a.y.b + h * a.y.h + row * a.y.s;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+            q[c] = load8<T>(rq, c * 16 + half * 8, s.DW, on);
+            go[c] = load8<T>(rg, c * 16 + half * 8, s.DW, on);
+            const Frag y = load8<T>(ry, c * 16 + half * 8, s.DW, on);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) delta += M::at(go[c], j) * M::at(y, j);
+        }
+        delta += other_half(delta);
+    }
+    float lse2 = __builtin_inff();                            // exp(x - inf) = 0: a query that sees nothing has no gradient
+    if (on) {
+        const float saved = a.lse[at];
+        if (saved != -__builtin_inff()) lse2 = saved * kLog2e;
+        if (half == 0) a.delta[at] = delta;
+    }
+    f32x16 acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
+    const float c2 = s.scale * kLog2e;
+
+    const Tiles t = tiles_of(s, r.length, r.start + i0, r.start + i1, KT);
+    Stage<T, DP, KT, 256> sk, sv;
+    if (t.n) {
+        const i32 j0 = tile_at(t, 0) * KT;
+        sk.load(K, a.k.s, j0, r.length, s.DW, tid);
+        sv.load(V, a.v.s, j0, r.length, s.DW, tid);
+    }
+    for (i32 n = 0; n < t.n; ++n) {
+        const i32 j0 = tile_at(t, n) * KT;
+        __syncthreads();
+        sk.store(ks, j0, r.length, s.DW, tid);
+        sv.store(vs, j0, r.length, s.DW, tid);
+        __syncthreads();
+        if (n + 1 < t.n) {
+            const i32 next = tile_at(t, n + 1) * KT;
+            sk.load(K, a.k.s, next, r.length, s.DW, tid);
+            sv.load(V, a.v.s, next, r.length, s.DW, tid);
+        }
+        if (w0 > w1) continue;
+#pragma unroll
+        for (int kb = 0; kb < KT / 32; ++kb) {
+            const i32 k0 = j0 + kb * 32;
+            if (none_visible(s, r.length, r.start + w0, r.start + w1, k0, k0 + 31)) continue;
+            f32x16 x = f32x16{}, dp = f32x16{};
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                x = M::run32(L::row(ks, kb * 32 + (lane & 31), 2 * c + half), q[c], x);
+                dp = M::run32(L::row(vs, kb * 32 + (lane & 31), 2 * c + half), go[c], dp);
+            }
+            const bool masked = !all_visible(s, r.length, r.start + w0, r.start + w1, k0, k0 + 31);
+            float e[16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                float w = exp2_of(x[v] * c2 - lse2) * (dp[v] - delta);
+                if (masked && !visible(s, r.length, p, k0 + 8 * (v >> 2) + 4 * half + (v & 3))) w = 0.0f;
+                e[v] = w;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const Frag ds = M::pack8(e + 8 * c);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] = M::run32(L::column(ks, kb * 32 + c * 16, d, lane), ds, acc[d]);
+            }
+        }
+    }
+    if (!on) return;
+    char* row = a.dq.p + (b * a.dq.b + h * a.dq.h + (u64)(u32)i * a.dq.s) * sizeof(T);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            put4<T>(row, a.dq.d, a.whole_dq, d * 32 + g * 8 + half * 4, s.D, acc[d][4 * g] * s.scale, acc[d][4 * g + 1] * s.scale, acc[d][4 * g + 2] * s.scale, acc[d][4 * g + 3] * s.scale);
+}
+
+// A wave keeps 32 keys and values in registers; the queries and gradients of every head of the group come by in tiles of QT
+// rows.  Here a lane is one key: P and dS, rounded, feed dv^T = grad^T P and dk^T = q^T dS as they lie.
+template <class T, int DP, int QT>
+__global__ __launch_bounds__(256) void attention_dkdv_k(BackwardArgs a)
+{
+    typedef Mma<T> M;
+    typedef typename M::Frag Frag;
+    typedef Tile<T, DP> L;
+    constexpr int DB = DP / 32, DC = DP / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char* qs = lds;
+    char* gs = lds + QT * L::PITCH;
+    float* ls = (float*)(lds + 2 * QT * L::PITCH);            // lse (log2), delta of the tile's rows
+    float* ds = ls + QT;
+    const Shape& s = a.s;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    const u32 id = xcd_order(blockIdx.x, gridDim.x), split = id % a.splits, rest = id / a.splits;
+    const u32 head = rest / a.tiles, tile = rest % a.tiles;
+    const u32 b = head / s.HK, hk = head % s.HK;
+    const Row r = row_of(s, b);
+    const i32 k0 = (i32)tile * 128, k1 = k0 + 127 < r.length - 1 ? k0 + 127 : r.length - 1;      // keys in use
+    const i32 j0 = k0 + wave * 32, j = j0 + (lane & 31);
+    const bool on = j < r.length;
+
+    Frag kf[DC], vf[DC];
+    {
+        const u64 row = (u64)(u32)(on ? j : 0);
+        const T* rk = (const T*)a.k.p + b * a.k.b + hk * a.k.h + row * a.k.s;
+        const T* rv = (const T*)a.v.p + b * a.v.b + hk * a.v.h + row * a.v.s;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) { kf[c] = load8<T>(rk, c * 16 + half * 8, s.DW, on); vf[c] = load8<T>(rv, c * 16 + half * 8, s.DW, on); }
+    }
+    f32x16 dk[DB], dv[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) { dk[d] = f32x16{}; dv[d] = f32x16{}; }
+    const float c2 = s.scale * kLog2e;
+
+    // the queries that can see a key of this block: positions [lo, hi)
+    i32 i_lo = 0, i_hi = 0;
+    if (k0 <= k1) {
+        i64 lo = s.causal ? k0 : 0, hi = (i64)r.start + s.SQ;
+        if (s.window && k0 >= s.sinks) {
+            if ((i64)k0 - s.window + 1 > lo) lo = (i64)k0 - s.window + 1;
+            if ((i64)k1 + s.window < hi) hi = (i64)k1 + s.window;
+        }
+        if (lo < r.start) lo = r.start;
+        if (lo < hi) { i_lo = (i32)(lo - r.start); i_hi = (i32)(hi - r.start); }
+    }
+    const i32 first = i_lo / QT, per = i_lo < i_hi ? (i_hi + QT - 1) / QT - first : 0;
+    const u64 total = (u64)(u32)per * s.G;
+    const u64 from = total * split / a.splits, to = total * (split + 1) / a.splits;
+
+    Stage<T, DP, QT, 256> sq, sg;
+    float next_l = 0.0f, next_d = 0.0f;
+    auto load = [&](u64 n) {
+        const u32 h = hk * s.G + (u32)(n / (u32)per);
+        const i32 i0 = (first + (i32)(n % (u32)per)) * QT;
+        sq.load((const T*)a.q.p + b * a.q.b + h * a.q.h, a.q.s, i0, s.SQ, s.DW, tid);
+        sg.load((const T*)a.grad.p + b * a.grad.b + h * a.grad.h, a.grad.s, i0, s.SQ, s.DW, tid);
+        if (tid < QT) {
+            const i32 i = i0 + tid < s.SQ ? i0 + tid : s.SQ - 1;
+            const u64 at = ((u64)b * s.H + h) * (u64)(u32)s.SQ + (u32)i;
+            const float saved = a.lse[at];
+            next_l = i0 + tid < s.SQ && saved != -__builtin_inff() ? saved * kLog2e : __builtin_inff();
+            next_d = a.delta[at];
+        }
+    };
+    if (from < to) load(from);
+    for (u64 n = from; n < to; ++n) {
+        const i32 i0 = (first + (i32)(n % (u32)per)) * QT;
+        __syncthreads();
+        sq.store(qs, i0, s.SQ, s.DW, tid);
+        sg.store(gs, i0, s.SQ, s.DW, tid);
+        if (tid < QT) { ls[tid] = next_l; ds[tid] = next_d; }
+        __syncthreads();
+        if (n + 1 < to) load(n + 1);
+#pragma unroll
+        for (int qb = 0; qb < QT / 32; ++qb) {
+            const i32 q0 = i0 + qb * 32, q1 = q0 + 31 < s.SQ ? q0 + 31 : s.SQ - 1;
+            if (q0 > q1 || none_visible(s, r.length, r.start + q0, r.start + q1, j0, j0 + 31)) continue;
+            f32x16 x = f32x16{}, dp = f32x16{};
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+                x = M::run32(L::row(qs, qb * 32 + (lane & 31), 2 * c + half), kf[c], x);
+                dp = M::run32(L::row(gs, qb * 32 + (lane & 31), 2 * c + half), vf[c], dp);
+            }
+            const bool masked = !all_visible(s, r.length, r.start + q0, r.start + q1, j0, j0 + 31);
+            float e[16], w[16];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 l4 = *(const f32x4*)(ls + qb * 32 + g * 8 + half * 4), d4 = *(const f32x4*)(ds + qb * 32 + g * 8 + half * 4);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    float y = exp2_of(x[4 * g + v] * c2 - l4[v]);
+                    float z = y * (dp[4 * g + v] - d4[v]);
+                    if (masked && !visible(s, r.length, r.start + q0 + 8 * g + 4 * half + v, j)) y = z = 0.0f;
+                    e[4 * g + v] = y;
+                    w[4 * g + v] = z;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const Frag fp = M::pack8(e + 8 * c), fs = M::pack8(w + 8 * c);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    dv[d] = M::run32(L::column(gs, qb * 32 + c * 16, d, lane), fp, dv[d]);
+                    dk[d] = M::run32(L::column(qs, qb * 32 + c * 16, d, lane), fs, dk[d]);
+                }
+            }
+        }
+    }
+    if (j >= s.SK) return;
+    if (a.splits > 1) {
+        const u64 rows = (u64)s.B * s.HK * (u32)s.SK, at = (u64)head * (u32)s.SK + (u32)j;
+        float* pk = a.part + ((u64)split * 2 * rows + at) * DP;
+        float* pv = pk + rows * DP;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = d * 32 + g * 8 + half * 4;
+                *(f32x4*)(pk + c) = f32x4{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
+                *(f32x4*)(pv + c) = f32x4{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
+            }
+        return;
+    }
+    char* rk = a.dk.p + (b * a.dk.b + hk * a.dk.h + (u64)(u32)j * a.dk.s) * sizeof(T);
+    char* rv = a.dv.p + (b * a.dv.b + hk * a.dv.h + (u64)(u32)j * a.dv.s) * sizeof(T);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const u32 c = d * 32 + g * 8 + half * 4;
+            put4<T>(rk, a.dk.d, a.whole_dk, c, s.D, dk[d][4 * g] * s.scale, dk[d][4 * g + 1] * s.scale, dk[d][4 * g + 2] * s.scale, dk[d][4 * g + 3] * s.scale);
+            put4<T>(rv, a.dv.d, a.whole_dv, c, s.D, dv[d][4 * g] * 1.0f, dv[d][4 * g + 1] * 1.0f, dv[d][4 * g + 2] * 1.0f, dv[d][4 * g + 3] * 1.0f);
+        }
+}
+
+// the shares of the queries added up in their order
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attention_dkdv_join_k(BackwardArgs a)
+{
+    constexpr int LANES = DP / 4;
+    const Shape& s = a.s;
+    const u64 rows = (u64)s.B * s.HK * (u32)s.SK;
+    const u64 row = (u64)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const u32 c = threadIdx.x % LANES * 4;
+    if (row >= rows) return;
+    f32x4 k = f32x4{}, v = f32x4{};
+    for (u32 n = 0; n < a.splits; ++n) {
+        k += *(const f32x4*)(a.part + (((u64)n * 2) * rows + row) * DP + c);
+        v += *(const f32x4*)(a.part + (((u64)n * 2 + 1) * rows + row) * DP + c);
+    }
+    const u64 j = row % (u32)s.SK, head = row / (u32)s.SK, hk = head % s.HK, b = head / s.HK;
+    put4<T>(a.dk.p + (b * a.dk.b + hk * a.dk.h + j * a.dk.s) * sizeof(T), a.dk.d, a.whole_dk, c, s.D, k.x * s.scale, k.y * s.scale, k.z * s.scale, k.w * s.scale);
+    put4<T>(a.dv.p + (b * a.dv.b + hk * a.dv.h + j * a.dv.s) * sizeof(T), a.dv.d, a.whole_dv, c, s.D, v.x, v.y, v.z, v.w);
+}
+
+template <class T, int DP> int backward(aixk_ctx* ctx, const Call& c, BackwardArgs a)
+{
+    const Shape& s = c.s;
+    // rows per LDS tile: 32 where 64 would leave less than two workgroups' worth of registers or LDS
+    constexpr int KT = DP * sizeof(T) <= 256 ? 64 : 32;
+    if (s.SQ > 0 && s.B > 0 && s.H > 0) {
+        a.tiles = ((u32)s.SQ + 127) / 128;
+        const u64 grid = (u64)s.B * s.H * a.tiles;
+        AIXK_REQUIRE(grid < (1ull << 31), "attention_backward: too many rows");
+        constexpr size_t lds = 2 * (size_t)KT * DP * sizeof(T);
+        AIXK_TRY(allow_lds(attention_dq_k<T, DP, KT>, lds));
+        hipLaunchKernelGGL((attention_dq_k<T, DP, KT>), dim3((unsigned)grid), dim3(256), lds, ctx->stream, a);
+        AIXK_HIP(hipGetLastError());
+    }
+    if (s.SK == 0 || s.B == 0 || s.HK == 0) return AIXK_OK;
+    a.tiles = ((u32)s.SK + 127) / 128;
+    const u64 grid = (u64)s.B * s.HK * a.tiles, rows = (u64)s.B * s.HK * (u32)s.SK;
+    // Shares of the queries until there are two workgroups per compute unit, each of at least 512 queries.
+    u64 splits = ((u64)ctx->cus * 2 + grid - 1) / grid;
+    const u64 most = ((u64)s.G * (u32)s.SQ + 511) / 512;
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+    AIXK_REQUIRE(grid * splits < (1ull << 31), "attention_backward: too many rows");
+    a.splits = (u32)splits;
+    if (splits > 1) {
+        void* ws;
+        AIXK_TRY(block_scratch(ctx, kScratchParts, (size_t)splits * 2 * rows * DP * sizeof(float), &ws));
+        a.part = (float*)ws;
+    }
+    constexpr size_t lds = 2 * (size_t)KT * DP * sizeof(T) + 2 * KT * sizeof(float);
+    AIXK_TRY(allow_lds(attention_dkdv_k<T, DP, KT>, lds));
+    hipLaunchKernelGGL((attention_dkdv_k<T, DP, KT>), dim3((unsigned)(grid * splits)), dim3(256), lds, ctx->stream, a);
+    AIXK_HIP(hipGetLastError());
+    if (splits > 1) {
+        constexpr u32 per = 256 / (DP / 4);
+        hipLaunchKernelGGL((attention_dkdv_join_k<T, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, ctx->stream, a);
+        AIXK_HIP(hipGetLastError());
+    }
+    return AIXK_OK;
+}
+
+} // namespace
+
+extern "C" int32_t aixk_attention_backward(aixk_ctx* ctx, const aixhip_tensor* grad, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* v,
+                                           const aixhip_tensor* out, const aixhip_tensor* lse, const aixk_attention_spec* spec,
+                                           const aixhip_tensor* dq, const aixhip_tensor* dk, const aixhip_tensor* dv)
+{
+    const char* what = "attention_backward";
+    Call c;
+    AIXK_TRY(c.shape(what, q, k, v, spec));
+    for (const aixhip_tensor* t : {grad, out}) {
+        AIXK_REQUIRE(valid_tensor(t) && t->rank == 4 && t->dtype == c.dtype && t->size == numel(t), "%s: bad descriptor of grad or out", what);
+        for (int d = 0; d < 4; ++d) AIXK_REQUIRE(t->shape[d] == q->shape[d], "%s: grad and out must have the shape of the queries", what);
+    }
+    AIXK_REQUIRE(lse != nullptr, "%s: the forward pass's lse is needed", what);
+    AIXK_TRY(c.statistics(what, lse, q, &c.lse));
+    i32 wq = 0, wk = 0, wv = 0;
+    AIXK_TRY(c.result(what, dq, q, "dq", &c.dq, &wq));
+    AIXK_TRY(c.result(what, dk, k, "dk", &c.dk, &wk));
+    AIXK_TRY(c.result(what, dv, v, "dv", &c.dv, &wv));
+    const aixhip_tensor* inputs[] = {grad, q, k, v, out, lse, spec->lengths, spec->starts};
+    for (const aixhip_tensor* in : inputs)
+        AIXK_REQUIRE(!overlap(dq, in) && !overlap(dk, in) && !overlap(dv, in), "%s: a result overlaps an operand", what);
+    // (the three may be interleaved views of one buffer, but not the same one)
+    auto same = [](const aixhip_tensor* x, const View& vx, const aixhip_tensor* y, const View& vy) { return numel(x) && numel(y) && vx.p == vy.p; };
+    AIXK_REQUIRE(!same(dq, c.dq, dk, c.dk) && !same(dq, c.dq, dv, c.dv) && !same(dk, c.dk, dv, c.dv), "%s: results share their memory", what);
+    AIXK_TRY(set_device(ctx));
+    AIXK_TRY(c.operand(ctx, q, kScratchQ, &c.q));
+    AIXK_TRY(c.operand(ctx, k, kScratchK, &c.k));
+    AIXK_TRY(c.operand(ctx, v, kScratchV, &c.v));
+    AIXK_TRY(c.operand(ctx, grad, kScratchGrad, &c.grad));
+    AIXK_TRY(c.operand(ctx, out, kScratchOut, &c.y));
+    void* delta;
+    AIXK_TRY(block_scratch(ctx, kScratchDelta, (size_t)(numel(lse) + 1) * sizeof(float), &delta));
+    BackwardArgs a{c.s, c.grad, c.q, c.k, c.v, c.y, c.dq, c.dk, c.dv, c.lse, (float*)delta, 0, 1, wq, wk, wv, nullptr};
+    return c.by_type([&](auto type, auto width) { return backward<decltype(type), decltype(width)::value>(ctx, c, a); });
+}

@@ -70,6 +70,12 @@ struct aixk_ctx {
     // like everything else
     void* gemm_ws[3]{nullptr, nullptr, nullptr};
     size_t gemm_ws_bytes[3]{0, 0, 0};
+    // scratch of the transformer-block operators by purpose (copies of operands, shares of a split sum), grown on demand
+    void* block_ws[12]{};
+    size_t block_ws_bytes[12]{};
+    // outgrown workspaces that a captured graph may still read and write: kept until the context goes
+    std::vector<void*> retired;
+    bool ever_captured{false};
     // small tables that kernels read from device memory (the operand addresses of a grouped launch): a pinned host ring
     // and its device twin, filled slot by slot and copied on the stream; an event per lap guards the reuse of a slot
     char* table_host{nullptr};
@@ -107,6 +113,16 @@ int resolve_static_scratch(aixk_ctx* ctx);
 // runtime.hip: `bytes` of table space: where the host writes it and where kernels will find it once table_upload() has run
 int table_slot(aixk_ctx* ctx, size_t bytes, void** host, const void** dev);
 int table_upload(aixk_ctx* ctx, const void* host, const void* dev, size_t bytes);          // reduce.hip; called once per context by aixk_create
+
+// runtime.hip: a workspace of at least `bytes`.  Grows on demand (never inside a capture); a buffer that a captured graph may
+// use is kept when it is outgrown.  All use is ordered on the context's single stream.
+int grow_workspace(aixk_ctx* ctx, void** buffer, size_t* have, size_t bytes);
+inline int block_scratch(aixk_ctx* ctx, int slot, size_t bytes, void** out)
+{
+    const int rc = grow_workspace(ctx, &ctx->block_ws[slot], &ctx->block_ws_bytes[slot], bytes);
+    *out = ctx->block_ws[slot];
+    return rc;
+}
 
 inline int set_device(aixk_ctx* ctx)
 {

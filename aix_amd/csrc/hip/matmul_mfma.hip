@@ -1554,18 +1554,7 @@ __global__ __launch_bounds__(256) void gemm_nt32_k(GemmArgs g, SplitArgs sk, con
 // context (all use is ordered on the context's single stream).
 int workspace(aixk_ctx* ctx, int which, size_t bytes, void** out)
 {
-    if (ctx->gemm_ws_bytes[which] < bytes) {
-        if (ctx->capturing) return fail(AIXK_EINVAL, "matmul workspace would have to grow inside a capture: run the same step once before capturing it");
-        if (ctx->gemm_ws[which]) {
-            AIXK_HIP(hipStreamSynchronize(ctx->stream));
-            AIXK_HIP(hipFree(ctx->gemm_ws[which]));
-            ctx->gemm_ws[which] = nullptr;
-            ctx->gemm_ws_bytes[which] = 0;
-        }
-        const size_t want = (bytes + (size_t(1) << 20)) & ~((size_t(1) << 20) - 1);
-        if (hipMalloc(&ctx->gemm_ws[which], want) != hipSuccess) { (void)hipGetLastError(); ctx->gemm_ws[which] = nullptr; return fail(AIXK_ENOMEM, "matmul workspace of %zu bytes", want); }
-        ctx->gemm_ws_bytes[which] = want;
-    }
+    AIXK_TRY(grow_workspace(ctx, &ctx->gemm_ws[which], &ctx->gemm_ws_bytes[which], bytes));
     *out = ctx->gemm_ws[which];
     return AIXK_OK;
 }

@@ -100,6 +100,28 @@ int table_upload(aixk_ctx* ctx, const void* host, const void* dev, size_t bytes)
     return AIXK_OK;
 }
 
+int grow_workspace(aixk_ctx* ctx, void** buffer, size_t* have, size_t bytes)
+{
+    if (*have >= bytes) return AIXK_OK;
+    if (ctx->capturing) return fail(AIXK_EINVAL, "a workspace would have to grow inside a capture: run the same step once before capturing it");
+    if (*buffer) {
+        if (ctx->ever_captured) {
+            // a graph captured before may name this buffer in its kernels' arguments; at least doubling bounds what is kept
+            try { ctx->retired.push_back(*buffer); } catch (...) { return fail(AIXK_ENOMEM, "out of host memory"); }
+            if (bytes < 2 * *have) bytes = 2 * *have;
+        } else {
+            AIXK_HIP(hipStreamSynchronize(ctx->stream));
+            AIXK_HIP(hipFree(*buffer));
+        }
+        *buffer = nullptr;
+        *have = 0;
+    }
+    const size_t want = (bytes + (size_t(1) << 20) - 1) & ~((size_t(1) << 20) - 1);
+    if (hipMalloc(buffer, want) != hipSuccess) { (void)hipGetLastError(); *buffer = nullptr; return fail(AIXK_ENOMEM, "workspace of %zu bytes", want); }
+    *have = want;
+    return AIXK_OK;
+}
+
 size_t stream_store_min_bytes()
 {
     static const size_t value = [] {
@@ -175,6 +197,8 @@ int32_t aixk_destroy(aixk_ctx* ctx)
     (void)hipFree(ctx->scratch);
     (void)hipFree(ctx->counter);
     for (void* ws : ctx->gemm_ws) if (ws) (void)hipFree(ws);
+    for (void* ws : ctx->block_ws) if (ws) (void)hipFree(ws);
+    for (void* ws : ctx->retired) (void)hipFree(ws);
     if (ctx->capturing) (void)aixk_capture_abort(ctx);
     if (ctx->side) (void)hipStreamDestroy(ctx->side);
     (void)hipStreamDestroy(ctx->stream);
@@ -498,6 +522,7 @@ int32_t aixk_capture_begin(aixk_ctx* ctx)
     // relaxed: the thread may go on calling hipMalloc and copying on other streams while this one records
     AIXK_HIP(hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeRelaxed));
     ctx->capturing = new aixk_graph();
+    ctx->ever_captured = true;
     return AIXK_OK;
 }
 

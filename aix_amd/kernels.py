@@ -19,6 +19,23 @@ class Tensor(C.Structure):
                 ("shape", C.c_uint64 * MAX_RANK), ("strides", C.c_uint64 * MAX_RANK)]
 
 
+def tensor(ptr, dtype, shape, strides=None, offset=0):
+    """A descriptor over device memory: strides and offset in elements, row-major if no strides are given."""
+    t = Tensor()
+    t.data, t.dtype, t.rank, t.offset = ptr, dtype, len(shape), offset
+    size = 1
+    for e in shape:
+        size *= e
+    if strides is None:
+        strides, run = [0] * len(shape), 1
+        for d in reversed(range(len(shape))):
+            strides[d], run = run, run * shape[d]
+    t.size = size
+    t.shape[:len(shape)] = shape
+    t.strides[:len(shape)] = strides
+    return t
+
+
 class FillItem(C.Structure):
     """aixk_fill_item"""
     _fields_ = [("dst", C.c_void_p), ("bits", C.c_uint64), ("elements", C.c_uint32), ("element_size", C.c_uint32)]
@@ -42,6 +59,12 @@ class ColsumItem(C.Structure):
 class PartialsItem(C.Structure):
     """aixk_partials_item"""
     _fields_ = [("partials", C.c_void_p), ("count", C.c_uint64), ("dst", Tensor), ("init_bits", C.c_uint64)]
+
+
+class AttentionSpec(C.Structure):
+    """aixk_attention_spec"""
+    _fields_ = [("scale", C.c_float), ("causal", C.c_int32), ("window", C.c_uint64), ("sinks", C.c_uint64),
+                ("lengths", C.POINTER(Tensor)), ("starts", C.POINTER(Tensor))]
 
 
 class DeviceInfo(C.Structure):
@@ -103,6 +126,8 @@ _SIGNATURES = {
     "aixk_mfma_only_rate": [_P, C.c_int32, C.c_int32, _P, C.c_uint32, C.c_double, C.POINTER(C.c_float), C.POINTER(C.c_float)],
     "aixk_matmul_batched": [_P, _T, _T, _T],
     "aixk_matmul_grouped": [_P, _T, _T, _T, C.c_uint32],
+    "aixk_attention": [_P, _T, _T, _T, C.POINTER(AttentionSpec), _T, _T],
+    "aixk_attention_backward": [_P, _T, _T, _T, _T, _T, _T, C.POINTER(AttentionSpec), _T, _T, _T],
     "aixk_rtc_get": [_P, C.c_char_p, C.c_char_p, C.c_char_p, C.POINTER(_P), C.POINTER(C.c_int32)],
     "aixk_rtc_launch": [_P, _P, C.c_uint32, C.c_uint32, _P, C.c_size_t],
     "aixk_rtc_launch_many": [_P, _P, C.c_uint32, _P, C.c_size_t, C.c_size_t, C.c_uint32],

@@ -227,6 +227,40 @@ int32_t aixk_matmul_batched(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_
  * chip one by one run as ONE launch; anything else one by one, with the result of aixk_matmul for every product. */
 int32_t aixk_matmul_grouped(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, uint32_t count);
 
+/* ---- operators of transformer blocks (no counterpart in the reference, which composes them from the operators above) ---- */
+/* What these share: element types f32, f16 and bf16 (one per call), sums, softmax statistics and norms in f32, one rounding
+ * per result unless stated.  Operands are any views; results are addressed through their offset and strides (like
+ * aixk_slice_set's), may not be broadcast views and may not overlap an operand unless stated.  Operand and result memory
+ * may be any device memory of the context's GPU whose earlier use the caller has ordered before the context's stream.
+ * The calls allocate nothing but workspaces of the context that grow on demand (inside a capture: AIXK_EINVAL if one would
+ * have to grow; run the same call once before). */
+
+/* Which keys a query sees.  Query i of sequence b stands at position p = starts[b] + i; it sees key j when
+ *   0 <= p,  j < lengths[b],  (causal: j <= p),  (window > 0: |p - j| < window, or j < sinks).
+ * lengths NULL: every key; starts NULL: the queries are the last ones, starts[b] = lengths[b] - queries.  Both are int32
+ * [batch] in device memory, read when the kernels run (a captured call follows their current values); lengths beyond the
+ * keys count as all of them, negative ones as none; starts are taken within +- 2^29.  Keys at and behind a length are never
+ * read.  A query that sees no key gives zeros and lse = -infinity, and no gradient. */
+typedef struct aixk_attention_spec {
+    float    scale;                  /* factor of the scores, positive and finite */
+    int32_t  causal;
+    uint64_t window;                 /* 0: none */
+    uint64_t sinks;                  /* leading keys that a window does not hide */
+    const aixhip_tensor* lengths;    /* or NULL */
+    const aixhip_tensor* starts;     /* or NULL */
+} aixk_attention_spec;
+/* out = softmax(scale q k^T, masked) v.  q, out: [batch, heads, queries, head dim]; k, v: [batch, key heads, keys, head dim],
+ * heads a multiple of key heads (query head h uses key head h / (heads / key heads)), head dim 1 .. 256; lse (or NULL): dense
+ * f32 [batch, heads, queries], the natural logarithm of every query's sum of exponentials, for the backward pass.
+ * The weights are rounded to the element type before they multiply v (the matrix unit's operand type). */
+int32_t aixk_attention(aixk_ctx* ctx, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* v, const aixk_attention_spec* spec,
+                       const aixhip_tensor* out, const aixhip_tensor* lse);
+/* The gradients of the above: grad and out like q, lse as aixk_attention left it; dq like q, dk and dv like k.  Key heads
+ * shared by several query heads receive the sum over them.  No atomics: results repeat bit for bit. */
+int32_t aixk_attention_backward(aixk_ctx* ctx, const aixhip_tensor* grad, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* v,
+                                const aixhip_tensor* out, const aixhip_tensor* lse, const aixk_attention_spec* spec,
+                                const aixhip_tensor* dq, const aixhip_tensor* dk, const aixhip_tensor* dv);
+
 /* ---- runtime-compiled fused elementwise kernels ------------------------- */
 /* Compile `source` (HIP C++, one extern "C" __global__ named `entry`) for gfx950 with hipRTC or
  * return the cached module for `key`.  *was_cached tells which.  Replaces the reference's
