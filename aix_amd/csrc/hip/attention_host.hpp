@@ -10,19 +10,9 @@ namespace aixk {
 namespace attn {
 
 // slots of the context's scratch memory (block_scratch)
-enum { kScratchQ = 0, kScratchK, kScratchV, kScratchGrad, kScratchOut, kScratchParts, kScratchDelta };
+enum { kScratchQ = 0, kScratchK, kScratchV, kScratchGrad, kScratchOut, kScratchParts, kScratchDelta, kScratchProduct, kScratchColumns };
 
 int pack(aixk_ctx* ctx, int dtype, const View& src, void* dst, u32 B, u32 H, u64 S, u32 D, u32 DW);      // attention.hip
-
-// Two views may share memory: their extents in bytes meet.
-inline bool overlap(const aixhip_tensor* a, const aixhip_tensor* b)
-{
-    if (!a || !b || numel(a) == 0 || numel(b) == 0) return false;
-    const size_t ea = aixk_dtype_size(a->dtype), eb = aixk_dtype_size(b->dtype);
-    const char *a0 = (const char*)a->data + a->offset * ea, *a1 = (const char*)a->data + view_extent(a) * ea;
-    const char *b0 = (const char*)b->data + b->offset * eb, *b1 = (const char*)b->data + view_extent(b) * eb;
-    return a0 < b1 && b0 < a1;
-}
 
 struct Call {
     Shape s{};

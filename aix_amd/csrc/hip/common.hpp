@@ -252,6 +252,16 @@ inline uint64_t view_extent(const aixhip_tensor* t)
     return last + 1;
 }
 
+// Two views may share memory: their extents in bytes meet.
+inline bool overlap(const aixhip_tensor* a, const aixhip_tensor* b)
+{
+    if (!a || !b || numel(a) == 0 || numel(b) == 0) return false;
+    const size_t ea = aixk_dtype_size(a->dtype), eb = aixk_dtype_size(b->dtype);
+    const char *a0 = (const char*)a->data + a->offset * ea, *a1 = (const char*)a->data + view_extent(a) * ea;
+    const char *b0 = (const char*)b->data + b->offset * eb, *b1 = (const char*)b->data + view_extent(b) * eb;
+    return a0 < b1 && b0 < a1;
+}
+
 inline unsigned grid_for(uint64_t work_items, unsigned per_block, unsigned max_blocks)
 {
     uint64_t b = (work_items + per_block - 1) / per_block;

@@ -14,9 +14,10 @@ using namespace aixd;
 using namespace aixk;
 
 namespace aixk {
+struct EpiArgs;
 // Implemented in matmul_mfma.hip.  Returns AIXK_OK if it launched, -1 if the shape/layout is not
 // one it handles (caller falls back), or an error status.
-int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out);
+int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const EpiArgs* epi);
 // The same for a stack of products (a, b, out: the 2-D descriptors of the first matrices; batch: the joint
 // collapsed space of the leading dims, operands a, b, out).
 int matmul_mfma_batched(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const Space<3>& batch);
@@ -112,7 +113,7 @@ extern "C" int32_t aixk_matmul(aixk_ctx* ctx, const aixhip_tensor* a, const aixh
     ctx->gemm_last_route = 0;
 
     if (out->dtype == AIXK_F32 || out->dtype == AIXK_F16 || out->dtype == AIXK_BF16) {
-        const int rc = matmul_mfma(ctx, a, b, out);
+        const int rc = matmul_mfma(ctx, a, b, out, nullptr);
         if (rc != -1) return rc;
     }
     const uint64_t gx = (N + TN - 1) / TN, gy = (M + TM - 1) / TM;

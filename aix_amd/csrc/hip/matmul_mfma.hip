@@ -32,6 +32,8 @@
 #pragma clang fp contract(fast)
 
 #include "common.hpp"
+#include "attention_host.hpp"
+#include "epilogue.hpp"
 
 #include <cstdio>
 #include <cstdlib>
@@ -104,6 +106,22 @@ template <> struct Mma16<f16> {
     static __device__ __forceinline__ u32 pack(float lo, float hi)
     { return (u32)__builtin_bit_cast(u16, (f16)lo) | ((u32)__builtin_bit_cast(u16, (f16)hi) << 16); }
 };
+
+// What a kernel without an epilogue takes in its place.
+struct NoEpi {};
+template <bool EPI> struct EpiOf { typedef NoEpi type; };
+template <> struct EpiOf<true> { typedef EpiArgs type; };
+// eight accumulated columns, with or without an epilogue, as a 16-byte word
+template <class T, bool EPI> __device__ __forceinline__ u32x4 finish8(f32x4 lo, f32x4 hi, const typename EpiOf<EPI>::type& e, u64 row, u64 col, u64 N)
+{
+    if constexpr (EPI) {
+        float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        epilogue8<T>(x, e, row, col, N);
+        lo = f32x4{x[0], x[1], x[2], x[3]};
+        hi = f32x4{x[4], x[5], x[6], x[7]};
+    }
+    return u32x4{Mma16<T>::pack(lo.x, lo.y), Mma16<T>::pack(lo.z, lo.w), Mma16<T>::pack(hi.x, hi.y), Mma16<T>::pack(hi.z, hi.w)};
+}
 
 // ---- 16-bit operands ---------------------------------------------------------------------------
 // BM x BN workgroup tile, BK = 64; LDS row = 64 elements + 8 padding = 144 bytes.
@@ -263,8 +281,8 @@ __device__ __forceinline__ u32x4 tr_fragment(const unsigned char* lds_addr)
 
 template <int N> struct Const { static constexpr int v = N; };
 
-template <class T, bool AT, bool BT>
-__global__ __launch_bounds__(512) void gemm_nt16_direct_k(GemmArgs g)
+template <class T, bool AT, bool BT, bool EPI = false>
+__global__ __launch_bounds__(512) void gemm_nt16_direct_k(GemmArgs g, typename EpiOf<EPI>::type epi)
 {
     constexpr int BM = 256, BK = 64, STAGE = 2 * 256 * BK * 2;      // 65536 bytes: A rows then B rows
     constexpr int WGN = 4, TI = 8, TJ = 4, WCOLS = TJ * 16;          // 2 x 4 waves of 128 x 64
@@ -389,10 +407,8 @@ __global__ __launch_bounds__(512) void gemm_nt16_direct_k(GemmArgs g)
             const int run = lane + 64 * t, row = run >> 3, cg = run & 7;
             const f32x4 lo = *(const f32x4*)(slab + row * PITCH + cg * 8);
             const f32x4 hi = *(const f32x4*)(slab + row * PITCH + cg * 8 + 4);
-            u32x4 o;
-            o.x = Mma16<T>::pack(lo.x, lo.y); o.y = Mma16<T>::pack(lo.z, lo.w);
-            o.z = Mma16<T>::pack(hi.x, hi.y); o.w = Mma16<T>::pack(hi.z, hi.w);
-            __builtin_nontemporal_store(o, (u32x4*)(C + (m0 + wm * 128 + i * 16 + row) * g.N + n0 + wn * WCOLS + cg * 8));
+            const u64 at_row = m0 + wm * 128 + i * 16 + row, at_col = n0 + wn * WCOLS + cg * 8;
+            __builtin_nontemporal_store(finish8<T, EPI>(lo, hi, epi, at_row, at_col, g.N), (u32x4*)(C + at_row * g.N + at_col));
         }
     }
 }
@@ -545,8 +561,8 @@ __global__ __launch_bounds__(256) void gemm_k64_nt_k(GemmArgs g, BatchArgs bt, u
 // f32; a lane whose accumulators hold an infinity or a NaN stores the launch's number into the flag word, as gemm_x3_k does.
 struct PlanesArgs { u64 plane_a, plane_b; u32* flag; u32 seq; };      // bytes from one plane to the next
 
-template <class T, bool AT, bool BT, int BM, int BN, bool PLANES = false>
-__global__ __launch_bounds__(512) void gemm_direct16_k(GemmArgs g, BatchArgs bt, PlanesArgs pl)
+template <class T, bool AT, bool BT, int BM, int BN, bool PLANES = false, bool EPI = false>
+__global__ __launch_bounds__(512) void gemm_direct16_k(GemmArgs g, BatchArgs bt, PlanesArgs pl, typename EpiOf<EPI>::type epi)
 {
     static_assert((BM == 128 && (BN == 128 || BN == 192 || BN == 256)) || (BM == 256 && BN == 256), "tiles this kernel is written for");
     static_assert(!PLANES || (!AT && !BT), "planes are laid out K-contiguous");
@@ -754,10 +770,8 @@ __global__ __launch_bounds__(512) void gemm_direct16_k(GemmArgs g, BatchArgs bt,
             if (RUNS % 64 == 0 || run < RUNS) {
                 const f32x4 lo = *(const f32x4*)(slab + row * PITCH + cg * 8);
                 const f32x4 hi = *(const f32x4*)(slab + row * PITCH + cg * 8 + 4);
-                u32x4 o;
-                o.x = Mma16<T>::pack(lo.x, lo.y); o.y = Mma16<T>::pack(lo.z, lo.w);
-                o.z = Mma16<T>::pack(hi.x, hi.y); o.w = Mma16<T>::pack(hi.z, hi.w);
-                __builtin_nontemporal_store(o, (u32x4*)(C + (m0 + wm * WROWS + i * 16 + row) * g.N + n0 + wn * WCOLS + cg * 8));
+                const u64 at_row = m0 + wm * WROWS + i * 16 + row, at_col = n0 + wn * WCOLS + cg * 8;
+                __builtin_nontemporal_store(finish8<T, EPI>(lo, hi, epi, at_row, at_col, g.N), (u32x4*)(C + at_row * g.N + at_col));
             }
         }
     }
@@ -922,8 +936,8 @@ template <int BM, int BN, int BK_, bool AT, bool BT> struct Tile16 {
     static constexpr size_t kLds = (size_t)2 * (SA + SB) * 2;
 };
 
-template <class T, int BM, int BN, int BKT, bool AT, bool BT, int RING = 0>
-__global__ __launch_bounds__(256) void gemm_tile16_k(GemmArgs g, BatchArgs bt, SplitArgs sk)
+template <class T, int BM, int BN, int BKT, bool AT, bool BT, int RING = 0, bool EPI = false>
+__global__ __launch_bounds__(256) void gemm_tile16_k(GemmArgs g, BatchArgs bt, SplitArgs sk, typename EpiOf<EPI>::type epi)
 {
     typedef Tile16<BM, BN, BKT, AT, BT> S;
     constexpr int BK = S::BK, PA = S::PA, PB = S::PB, SA = S::SA, SB = S::SB;
@@ -1087,7 +1101,9 @@ __global__ __launch_bounds__(256) void gemm_tile16_k(GemmArgs g, BatchArgs bt, S
     const u64 plane = g.M * g.N;
     T* C = bt.table ? global_ptr<T>(bt.table[3 * (u64)blockIdx.y + 2]) : (T*)g.c + (u64)blockIdx.y * plane;
     float* P = sk.splits > 1 ? sk.partial + ((u64)blockIdx.z * sk.matrices + blockIdx.y) * plane : nullptr;
-    if (!P && g.N % 8 == 0 && ((size_t)g.c & 15) == 0) {
+    bool whole = true;
+    if constexpr (EPI) whole = epi.whole;
+    if (!P && g.N % 8 == 0 && ((size_t)g.c & 15) == 0 && whole) {
         // Through LDS (free after the last barrier), each wave on its own 32 x 32 slab: written as the MFMA leaves it (a lane
         // = a column), read back as runs of 8 columns, rounded and stored 16 bytes per lane: an eighth of the store
         // instructions of two-byte stores straight from the accumulators (4-8 % of a [8192, 768] x [768, 768] product; the
@@ -1107,12 +1123,7 @@ __global__ __launch_bounds__(256) void gemm_tile16_k(GemmArgs g, BatchArgs bt, S
                     const f32x4 lo = *(const f32x4*)(slab + r * PITCH + cg * 8);
                     const f32x4 hi = *(const f32x4*)(slab + r * PITCH + cg * 8 + 4);
                     const u64 row = m0 + wm * WM + i * 32 + r, col = n0 + wn * WN + j * 32 + cg * 8;
-                    if (row < g.M && col < g.N) {
-                        u32x4 o;
-                        o.x = Mma16<T>::pack(lo.x, lo.y); o.y = Mma16<T>::pack(lo.z, lo.w);
-                        o.z = Mma16<T>::pack(hi.x, hi.y); o.w = Mma16<T>::pack(hi.z, hi.w);
-                        *(u32x4*)(C + row * g.N + col) = o;
-                    }
+                    if (row < g.M && col < g.N) *(u32x4*)(C + row * g.N + col) = finish8<T, EPI>(lo, hi, epi, row, col, g.N);
                 }
             }
         return;
@@ -1127,10 +1138,39 @@ __global__ __launch_bounds__(256) void gemm_tile16_k(GemmArgs g, BatchArgs bt, S
                 const u64 row = m0 + wm * WM + i * 32 + (v >> 2) * 8 + (lane >> 5) * 4 + (v & 3);
                 if (row < g.M && col < g.N) {
                     if (P) P[row * g.N + col] = acc[i][j][v];
+                    else if constexpr (EPI) C[row * g.N + col] = Mma16<T>::out(epilogue1<T>(acc[i][j][v], epi, row, col, g.N));
                     else C[row * g.N + col] = Mma16<T>::out(acc[i][j][v]);
                 }
             }
         }
+}
+
+// The same with an epilogue, eight columns per lane where they are whole: partial results of `splits` K splits (none: a
+// product over nothing), [split][M][N]; one split may be the f32 result itself, finished in place.
+template <class T>
+__global__ __launch_bounds__(256) void splitk_epilogue_k(const float* partial, T* out, u64 M, u64 N, u32 splits, EpiArgs epi)
+{
+    const u64 total = M * N, step = (u64)gridDim.x * 256;
+    if (epi.whole) {
+        for (u64 g = (u64)blockIdx.x * 256 + threadIdx.x; g < total / 8; g += step) {
+            const u64 e = g * 8, row = e / N, col = e % N;
+            float x[8] = {};
+            for (u32 s = 0; s < splits; ++s) {
+                float y[8];
+                get8(partial + (u64)s * total + e, y);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] += y[j];
+            }
+            epilogue8<T>(x, epi, row, col, N);
+            put8(out + e, x);
+        }
+        return;
+    }
+    for (u64 e = (u64)blockIdx.x * 256 + threadIdx.x; e < total; e += step) {
+        float x = 0.0f;
+        for (u32 s = 0; s < splits; ++s) x += partial[(u64)s * total + e];
+        out[e] = down<T>(epilogue1<T>(x, epi, e / N, e % N, N));
+    }
 }
 
 // out[e] = the partial results of all K splits added in split order, rounded once.
@@ -1628,10 +1668,21 @@ int launch_small16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b
 // the 128-row tiles 32 (more workgroups per compute unit; the transformer's shapes are 5 % faster overall).
 constexpr int tile16_bk(int bm) { return bm == 64 ? 64 : 32; }
 
+int launch_epilogue(aixk_ctx* ctx, const float* partial, const aixhip_tensor* out, u32 splits, const EpiArgs& epi)
+{
+    const uint64_t M = out->shape[0], N = out->shape[1];
+    const unsigned blocks = grid_for(epi.whole ? M * N / 8 : M * N, 256, (unsigned)ctx->cus * 16u);
+    if (out->dtype == AIXK_BF16) hipLaunchKernelGGL((splitk_epilogue_k<bf16>), dim3(blocks), dim3(256), 0, ctx->stream, partial, (bf16*)out->data, (u64)M, (u64)N, splits, epi);
+    else if (out->dtype == AIXK_F16) hipLaunchKernelGGL((splitk_epilogue_k<f16>), dim3(blocks), dim3(256), 0, ctx->stream, partial, (f16*)out->data, (u64)M, (u64)N, splits, epi);
+    else hipLaunchKernelGGL((splitk_epilogue_k<float>), dim3(blocks), dim3(256), 0, ctx->stream, partial, (float*)out->data, (u64)M, (u64)N, splits, epi);
+    AIXK_HIP(hipGetLastError());
+    return AIXK_OK;
+}
+
 // gemm_tile16_k on the last two dims of a / b, `batch` as for launch_small16.  tile: 0 = 64 x 64, 1 = 128 x 64,
 // 2 = 128 x 128, 3 = 128 x 192, 4 = 192 x 128; splits: K splits wanted (1 = none).  -1: a layout the kernel does not take.
 int launch_tile16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const Space<3>* batch,
-                  int tile, uint64_t splits, const u64* table = nullptr)
+                  int tile, uint64_t splits, const u64* table = nullptr, const EpiArgs* epi = nullptr)
 {
     const uint64_t M = a->shape[0], K = a->shape[1], N = b->shape[1];
     constexpr size_t esz = 2;
@@ -1679,9 +1730,28 @@ int launch_tile16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b,
     const bool at = !a_k, tb = !b_k;
     auto launch = [&](auto kernel, size_t lds) {
         AIXK_TRY(set_lds(kernel, lds));
-        hipLaunchKernelGGL(kernel, dim3(n, (unsigned)count, sk.splits), dim3(256), lds, ctx->stream, g, bt, sk);
+        hipLaunchKernelGGL(kernel, dim3(n, (unsigned)count, sk.splits), dim3(256), lds, ctx->stream, g, bt, sk, NoEpi{});
         AIXK_HIP(hipGetLastError());
         return (int)AIXK_OK;
+    };
+    // with an epilogue: tiles 0, 1 and 2, A K-contiguous (the caller has seen to it)
+    auto epi_by_form = [&](auto dtype_tag, auto bm_tag, auto bn_tag) {
+        typedef decltype(dtype_tag) T;
+        constexpr int BM = decltype(bm_tag)::value, BN = decltype(bn_tag)::value, BK = tile16_bk(BM);
+        auto go = [&](auto kernel, size_t lds) {
+            AIXK_TRY(set_lds(kernel, lds));
+            hipLaunchKernelGGL(kernel, dim3(n, (unsigned)count, sk.splits), dim3(256), lds, ctx->stream, g, bt, sk, *epi);
+            AIXK_HIP(hipGetLastError());
+            return (int)AIXK_OK;
+        };
+        if (at) return -1;
+        if (!tb) return go(gemm_tile16_k<T, BM, BN, BK, false, false, 0, true>, Tile16<BM, BN, BK, false, false>::kLds);
+        return go(gemm_tile16_k<T, BM, BN, BK, false, true, 0, true>, Tile16<BM, BN, BK, false, true>::kLds);
+    };
+    auto epi_by_tile = [&](auto dtype_tag) {
+        if (tile == 0) return epi_by_form(dtype_tag, std::integral_constant<int, 64>{}, std::integral_constant<int, 64>{});
+        if (tile == 1) return epi_by_form(dtype_tag, std::integral_constant<int, 128>{}, std::integral_constant<int, 64>{});
+        return epi_by_form(dtype_tag, std::integral_constant<int, 128>{}, std::integral_constant<int, 128>{});
     };
     auto by_form = [&](auto dtype_tag, auto bm_tag, auto bn_tag, auto bk_tag, auto ring_tag) {
         typedef decltype(dtype_tag) T;
@@ -1700,6 +1770,10 @@ int launch_tile16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b,
         if (tile == 4) return by_form(dtype_tag, std::integral_constant<int, 192>{}, std::integral_constant<int, 128>{}, usual, usual);
         return by_form(dtype_tag, std::integral_constant<int, 128>{}, std::integral_constant<int, 128>{}, usual, usual);
     };
+    if (epi) {
+        const int rc = out->dtype == AIXK_BF16 ? epi_by_tile(bf16{}) : epi_by_tile(f16{});
+        return rc != AIXK_OK || sk.splits == 1 ? rc : launch_epilogue(ctx, sk.partial, out, sk.splits, *epi);
+    }
     const int rc = out->dtype == AIXK_BF16 ? by_tile(bf16{}) : by_tile(f16{});
     if (rc != AIXK_OK || sk.splits == 1) return rc;
     const uint64_t total = count * M * N;
@@ -1763,7 +1837,8 @@ int launch_k64(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, co
 // on its smaller tiles (gemm_direct16_k).  `batch` / `table` as for launch_small16 (a stack of matrices, or a group of
 // separate products).  limit > 0: only if the estimated cost stays below it (the caller has another kernel to offer).
 // -1: not for this product.
-int launch_direct16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const Space<3>* batch, const u64* table, double limit)
+int launch_direct16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const Space<3>* batch, const u64* table, double limit,
+                    const EpiArgs* epi = nullptr)
 {
     const uint64_t M = a->shape[0], K = a->shape[1], N = b->shape[1];
     constexpr size_t esz = 2;
@@ -1823,10 +1898,30 @@ int launch_direct16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* 
     const bool at = !a_k, tb = !b_k;
     auto launch = [&](auto kernel) {
         AIXK_TRY(set_lds(kernel, lds));
-        hipLaunchKernelGGL(kernel, dim3(n, (unsigned)count), dim3(512), lds, ctx->stream, g, bt, PlanesArgs{});
+        hipLaunchKernelGGL(kernel, dim3(n, (unsigned)count), dim3(512), lds, ctx->stream, g, bt, PlanesArgs{}, NoEpi{});
         AIXK_HIP(hipGetLastError());
         return (int)AIXK_OK;
     };
+    if (epi) {                                             // a single product with an epilogue: A K-contiguous
+        if (at || bm != 128) return -1;
+        auto go = [&](auto kernel) {
+            AIXK_TRY(set_lds(kernel, lds));
+            hipLaunchKernelGGL(kernel, dim3(n, (unsigned)count), dim3(512), lds, ctx->stream, g, bt, PlanesArgs{}, *epi);
+            AIXK_HIP(hipGetLastError());
+            return (int)AIXK_OK;
+        };
+        auto with = [&](auto dtype_tag, auto bn_tag) {
+            typedef decltype(dtype_tag) T;
+            constexpr int BN = decltype(bn_tag)::value;
+            return tb ? go(gemm_direct16_k<T, false, true, 128, BN, false, true>) : go(gemm_direct16_k<T, false, false, 128, BN, false, true>);
+        };
+        auto wide = [&](auto dtype_tag) {
+            if (bn == 256) return with(dtype_tag, std::integral_constant<int, 256>{});
+            if (bn == 192) return with(dtype_tag, std::integral_constant<int, 192>{});
+            return with(dtype_tag, std::integral_constant<int, 128>{});
+        };
+        return out->dtype == AIXK_BF16 ? wide(bf16{}) : wide(f16{});
+    }
     auto by_form = [&](auto dtype_tag, auto bn_tag, auto bm_tag) {
         typedef decltype(dtype_tag) T;
         constexpr int BN = decltype(bn_tag)::value, BM = decltype(bm_tag)::value;
@@ -1850,7 +1945,8 @@ int launch_direct16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* 
 // [8192,768]x[768,768] 28 -> 23, [8192,3072]^T-free x [3072,768] 76 -> 67, weight gradients [768,8192]x[8192,768]
 // 73 -> 32 (8 K splits) and [768,8192]x[8192,3072] 113 -> 72 (4 splits), stacks of 192 attention products
 // [512,64]x[64,512] 121 -> 42, [512,512]x[512,64] 52 -> 27, [512,512]^T x [512,64] 92 -> 27.
-int route16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const Space<3>* batch, const u64* table = nullptr)
+int route16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const Space<3>* batch, const u64* table = nullptr,
+            const EpiArgs* epi = nullptr)
 {
     const uint64_t M = a->shape[0], K = a->shape[1], N = b->shape[1];
     const uint64_t cus = (uint64_t)ctx->cus;
@@ -1894,7 +1990,7 @@ int route16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const
         uint64_t splits = 1;
         int tile = 2;
         double least = 0.0;
-        for (int cand = 2; cand <= 4; ++cand) {
+        for (int cand = 2; cand <= (epi ? 2 : 4); ++cand) {
             if (cand == 3 && (N % 192 != 0 || M % 128 != 0)) continue;
             if (cand == 4 && (M % 192 != 0 || N % 128 != 0)) continue;
             const uint64_t tiles = cand == 2 ? t128 : cand == 3 ? (M / 128) * (N / 192) : (M / 192) * (N / 128);
@@ -1914,24 +2010,25 @@ int route16(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const
         int tile = 2;
         const uint64_t steps = (K + 31) / 32;
         const uint64_t splits = cheapest(std::max<uint64_t>(1, std::min<uint64_t>(steps / 16, 16)), &tile);
-        return launch_tile16(ctx, a, b, out, nullptr, tile, splits);
+        return launch_tile16(ctx, a, b, out, nullptr, tile, splits, nullptr, epi);
     }
     if (t64 < 2 * cus) {
         // outputs that 64 x 64 tiles cannot spread over the chip twice: with a long K, 64 x 64 tiles and K split over
         // workgroups; from half a tile per compute unit on, 64 x 64 tiles as they are (their interior tiles prefetch three K
         // steps ahead: 1024^3 NN 12.0 -> 8.7 us, [1024,1024] x K 2048 20.3 -> 13.3, 1280^3 TN 37.5 -> 14.2); below that, 32 x 32
         // tiles with K split over the waves (512^3: 4.3 us against 5.9)
-        if (K >= 4096) return launch_tile16(ctx, a, b, out, nullptr, 0, splits_for(t64, (K + 63) / 64 * 2, 4));
-        if (2 * t64 > cus) return launch_tile16(ctx, a, b, out, nullptr, 0, 1);
+        if (K >= 4096) return launch_tile16(ctx, a, b, out, nullptr, 0, splits_for(t64, (K + 63) / 64 * 2, 4), nullptr, epi);
+        if (2 * t64 > cus) return launch_tile16(ctx, a, b, out, nullptr, 0, 1, nullptr, epi);
+        if (epi) return launch_tile16(ctx, a, b, out, nullptr, 0, std::max<uint64_t>(1, std::min<uint64_t>((K + 255) / 256, cus / std::max<uint64_t>(1, t64))), nullptr, epi);
         return launch_small16(ctx, a, b, out, nullptr);
     }
     if (2 * t128 >= cus) {                                 // (2048^3: 256 tiles of 128 x 128 27.4 us, 512 of 128 x 64 33.0; 1536^3: 144 tiles 19.6, 576 of 64 x 64 22.1)
         int tile = 2;
         (void)cheapest(1, &tile);
-        return launch_tile16(ctx, a, b, out, nullptr, tile, 1);
+        return launch_tile16(ctx, a, b, out, nullptr, tile, 1, nullptr, epi);
     }
-    if (t12864 >= 2 * cus) return launch_tile16(ctx, a, b, out, nullptr, 1, 1);
-    return launch_tile16(ctx, a, b, out, nullptr, 0, 1);
+    if (t12864 >= 2 * cus) return launch_tile16(ctx, a, b, out, nullptr, 1, 1, nullptr, epi);
+    return launch_tile16(ctx, a, b, out, nullptr, 0, 1, nullptr, epi);
 }
 
 } // namespace
@@ -1980,22 +2077,23 @@ int matmul_mfma_grouped(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tens
     return route16(ctx, &a[0], &b[0], &o2, &batch, dev);
 }
 
-int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out)
+int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const EpiArgs* epi)
 {
     const uint64_t M = a->shape[0], K = a->shape[1], N = b->shape[1];
     const size_t esz = aixk_dtype_size(out->dtype);
     const uint64_t kq = 16 / esz;                                 // elements per 16-byte chunk
-    if (K % kq != 0 || M * N < 64 * 64) return -1;                // odd K / tiny outputs: LDS-tiled kernel
+    if (K % kq != 0 || (M * N < 64 * 64 && !epi)) return -1;      // odd K / tiny outputs: LDS-tiled kernel
     if (((M + 63) / 64) * ((N + 63) / 64) >= (1ull << 31)) return -1;
 
     // 16-bit, whole 256 x 256 x 64 tiles, enough of them: every operand layout is consumed where it lies
     // (K-contiguous, or "T" form with unit stride along M / N), no gathers.
-    if (esz == 2 && M % 256 == 0 && N % 256 == 0 && K % 64 == 0 && (M / 256) * (N / 256) >= (uint64_t)ctx->cus / 2 &&
+    const bool direct = !epi || epi->whole;                       // (the LDS-direct kernels finish eight columns at a time)
+    if (esz == 2 && direct && M % 256 == 0 && N % 256 == 0 && K % 64 == 0 && (M / 256) * (N / 256) >= (uint64_t)ctx->cus / 2 &&
         (M / 256) * (N / 256) < (1ull << 31)) {
         // unless smaller tiles fill the chip's rounds so much better that they win all the same ([8192, 768] x [768, 2304]:
         // 288 tiles are a full round and an eighth of one, 44.7 us; 768 tiles of 128 x 192 are three full rounds, 36-39 us)
         const uint64_t t256 = (M / 256) * (N / 256);
-        const int rc = launch_direct16(ctx, a, b, out, nullptr, nullptr, (double)(((t256 + (uint64_t)ctx->cus - 1) / (uint64_t)ctx->cus) * 65536));
+        const int rc = launch_direct16(ctx, a, b, out, nullptr, nullptr, (double)(((t256 + (uint64_t)ctx->cus - 1) / (uint64_t)ctx->cus) * 65536), epi);
         if (rc != -1) return rc;
         const char* qa = (const char*)a->data + a->offset * esz;
         const char* qb = (const char*)b->data + b->offset * esz;
@@ -2013,10 +2111,20 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
             const bool at = !a_k, bt = !b_k;
             auto launch = [&](auto kernel) {
                 AIXK_TRY(set_lds(kernel, lds));
-                hipLaunchKernelGGL(kernel, dim3(n), dim3(512), lds, ctx->stream, g);
+                hipLaunchKernelGGL(kernel, dim3(n), dim3(512), lds, ctx->stream, g, NoEpi{});
                 AIXK_HIP(hipGetLastError());
                 return (int)AIXK_OK;
             };
+            if (epi) {
+                auto go = [&](auto kernel) {
+                    AIXK_TRY(set_lds(kernel, lds));
+                    hipLaunchKernelGGL(kernel, dim3(n), dim3(512), lds, ctx->stream, g, *epi);
+                    AIXK_HIP(hipGetLastError());
+                    return (int)AIXK_OK;
+                };
+                if (out->dtype == AIXK_BF16) return bt ? go(gemm_nt16_direct_k<bf16, false, true, true>) : go(gemm_nt16_direct_k<bf16, false, false, true>);
+                return bt ? go(gemm_nt16_direct_k<f16, false, true, true>) : go(gemm_nt16_direct_k<f16, false, false, true>);
+            }
             if (out->dtype == AIXK_BF16) {
                 if (!at && !bt) return launch(gemm_nt16_direct_k<bf16, false, false>);
                 if (!at && bt) return launch(gemm_nt16_direct_k<bf16, false, true>);
@@ -2030,12 +2138,12 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
         }
     }
 
-    if (esz == 2) { const int rc = launch_direct16(ctx, a, b, out, nullptr, nullptr, 0); if (rc != -1) return rc; }
+    if (esz == 2 && direct) { const int rc = launch_direct16(ctx, a, b, out, nullptr, nullptr, 0, epi); if (rc != -1) return rc; }
 
     // 16-bit, operands consumed where they lie (K-contiguous or T form): tiles and K splits by shape
     if (esz == 2) {
-        const int rc = route16(ctx, a, b, out, nullptr);
-        if (rc != -1) return rc;
+        const int rc = route16(ctx, a, b, out, nullptr, nullptr, epi);
+        if (rc != -1 || epi) return rc;
     }
 
     auto grid_of = [&](GemmArgs& g, uint64_t bm, uint64_t bn) {
@@ -2109,7 +2217,7 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
             constexpr size_t lds = 2 * 65536;
             auto kernel = gemm_direct16_k<bf16, false, false, 256, 256, true>;
             AIXK_TRY(set_lds(kernel, lds));
-            hipLaunchKernelGGL(kernel, dim3(n), dim3(512), lds, ctx->stream, gp, BatchArgs{}, PlanesArgs{M * Kp * 2, N * Kp * 2, (u32*)ctx->counter, seq});
+            hipLaunchKernelGGL(kernel, dim3(n), dim3(512), lds, ctx->stream, gp, BatchArgs{}, PlanesArgs{M * Kp * 2, N * Kp * 2, (u32*)ctx->counter, seq}, NoEpi{});
             AIXK_HIP(hipGetLastError());
             only_if = (const u32*)ctx->counter;
             ctx->gemm_last_route = 1;
@@ -2244,6 +2352,48 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
     }
     AIXK_HIP(hipGetLastError());
     return AIXK_OK;
+}
+
+// A product with an epilogue.  16-bit operands: the kernels above finish their accumulators in place; A comes K-contiguous
+// and both with whole 16-byte words along K, anything else is copied first.  f32: the product as aixk_matmul forms it, then
+// one pass over the result.
+int matmul_mfma_epilogue(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const EpiArgs& epi)
+{
+    const uint64_t M = a->shape[0], K = a->shape[1], N = b->shape[1];
+    if (K == 0) return launch_epilogue(ctx, nullptr, out, 0, epi);
+    if (out->dtype == AIXK_F32) {
+        aixhip_tensor product = *out;
+        if (epi.res && epi.res == out->data) {                    // the residual lies where the product would go
+            void* ws;
+            AIXK_TRY(block_scratch(ctx, attn::kScratchProduct, (size_t)(M * N) * sizeof(float), &ws));
+            product.data = ws;
+        }
+        AIXK_TRY(aixk_matmul(ctx, a, b, &product));
+        return launch_epilogue(ctx, (const float*)product.data, out, 1, epi);
+    }
+    constexpr size_t esz = 2;
+    const char* qa = (const char*)a->data + a->offset * esz;
+    const char* qb = (const char*)b->data + b->offset * esz;
+    const uint64_t Kp = (K + 7) / 8 * 8;
+    aixhip_tensor ta = *a, tb = *b;
+    if (K != Kp || a->strides[1] != 1 || (M > 1 && a->strides[0] % 8 != 0) || !aligned16(qa)) {
+        AIXK_REQUIRE(Kp < (1ull << 31), "matmul_epilogue: shape too large");
+        void* ws;
+        AIXK_TRY(workspace(ctx, 0, M * Kp * esz, &ws));
+        AIXK_TRY(attn::pack(ctx, out->dtype, attn::View{(char*)qa, 0, 0, a->strides[0], a->strides[1]}, ws, 1, 1, M, (u32)K, (u32)Kp));
+        ta.data = ws; ta.offset = 0; ta.strides[0] = Kp; ta.strides[1] = 1;
+    } else if (M == 1) ta.strides[0] = Kp;
+    const bool b_k = b->strides[0] == 1 && (N == 1 || b->strides[1] % 8 == 0), b_n = b->strides[1] == 1 && N % 8 == 0 && b->strides[0] % 8 == 0;
+    if (K != Kp || !(b_k || b_n) || !aligned16(qb)) {
+        AIXK_REQUIRE(Kp < (1ull << 31), "matmul_epilogue: shape too large");
+        void* ws;
+        AIXK_TRY(workspace(ctx, 1, N * Kp * esz, &ws));
+        AIXK_TRY(attn::pack(ctx, out->dtype, attn::View{(char*)qb, 0, 0, b->strides[1], b->strides[0]}, ws, 1, 1, N, (u32)K, (u32)Kp));
+        tb.data = ws; tb.offset = 0; tb.strides[0] = 1; tb.strides[1] = Kp;
+    } else if (N == 1) tb.strides[1] = Kp;
+    ta.shape[1] = Kp; tb.shape[0] = Kp;
+    const int rc = matmul_mfma(ctx, &ta, &tb, out, &epi);
+    return rc == -1 ? fail(AIXK_EINVAL, "matmul_epilogue: no kernel takes these operands") : rc;
 }
 
 } // namespace aixk

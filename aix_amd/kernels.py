@@ -9,6 +9,8 @@ F64, F32, F16, BF16, I64, I32, I16, I8, U8 = range(9)
 ADD, SUB, MUL, DIV, POW = range(5)
 NEG, SQRT, SIN, COS, TANH, LOG, EXP = range(7)
 SUM, MAX, ARGMAX, ARGMAX_ONEHOT = range(4)
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_PARTS = range(4)
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = range(4)
 MEM_DEVICE, MEM_MANAGED, MEM_PINNED = range(3)
 
 
@@ -65,6 +67,17 @@ class AttentionSpec(C.Structure):
     """aixk_attention_spec"""
     _fields_ = [("scale", C.c_float), ("causal", C.c_int32), ("window", C.c_uint64), ("sinks", C.c_uint64),
                 ("lengths", C.POINTER(Tensor)), ("starts", C.POINTER(Tensor))]
+
+
+class RotarySpec(C.Structure):
+    """aixk_rotary_spec"""
+    _fields_ = [("dims", C.c_uint32), ("interleaved", C.c_int32), ("inverse", C.c_int32), ("scaling", C.c_int32), ("base", C.c_double), ("factor", C.c_double),
+                ("original_length", C.c_double), ("low_turns", C.c_double), ("high_turns", C.c_double), ("magnitude", C.c_float)]
+
+
+class Epilogue(C.Structure):
+    """aixk_epilogue"""
+    _fields_ = [("bias", C.POINTER(Tensor)), ("residual", C.POINTER(Tensor)), ("pre", C.POINTER(Tensor)), ("activation", C.c_int32)]
 
 
 class DeviceInfo(C.Structure):
@@ -128,6 +141,9 @@ _SIGNATURES = {
     "aixk_matmul_grouped": [_P, _T, _T, _T, C.c_uint32],
     "aixk_attention": [_P, _T, _T, _T, C.POINTER(AttentionSpec), _T, _T],
     "aixk_attention_backward": [_P, _T, _T, _T, _T, _T, _T, C.POINTER(AttentionSpec), _T, _T, _T],
+    "aixk_rotary": [_P, _T, _T, _T, C.POINTER(RotarySpec), _T, _T],
+    "aixk_matmul_epilogue": [_P, _T, _T, C.POINTER(Epilogue), _T],
+    "aixk_matmul_epilogue_backward": [_P, _T, _T, _T, _T, C.c_int32, _T, _T, _T, _T],
     "aixk_rtc_get": [_P, C.c_char_p, C.c_char_p, C.c_char_p, C.POINTER(_P), C.POINTER(C.c_int32)],
     "aixk_rtc_launch": [_P, _P, C.c_uint32, C.c_uint32, _P, C.c_size_t],
     "aixk_rtc_launch_many": [_P, _P, C.c_uint32, _P, C.c_size_t, C.c_size_t, C.c_uint32],

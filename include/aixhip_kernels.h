@@ -261,6 +261,44 @@ int32_t aixk_attention_backward(aixk_ctx* ctx, const aixhip_tensor* grad, const 
                                 const aixhip_tensor* out, const aixhip_tensor* lse, const aixk_attention_spec* spec,
                                 const aixhip_tensor* dq, const aixhip_tensor* dk, const aixhip_tensor* dv);
 
+/* Rotary positions: of every head's first `dims` elements, pair i is turned by position * f_i, the other elements are copied.
+ * f_i = base^(-2 i / dims), for longer contexts than a model was trained on divided by `factor` (LINEAR), taken from the base
+ * base * factor^(dims / (dims - 2)) (BASE), or divided by `factor` only where a pair turns little over the original length
+ * (PARTS): with n_i = original_length f_i / (2 pi) and kept = clamp((n_i - low_turns) / (high_turns - low_turns), 0, 1),
+ * f_i (kept + (1 - kept) / factor).  Cosines and sines are multiplied by `magnitude` (1: none). */
+enum aixk_rotary_scaling { AIXK_ROTARY_PLAIN = 0, AIXK_ROTARY_LINEAR = 1, AIXK_ROTARY_BASE = 2, AIXK_ROTARY_PARTS = 3 };
+typedef struct aixk_rotary_spec {
+    uint32_t dims;                   /* even, 2 .. 256, at most the head dim */
+    int32_t  interleaved;            /* pairs (2 i, 2 i + 1); 0: (i, i + dims / 2) */
+    int32_t  inverse;                /* turn back: the gradient of the operator is the inverse turn of the result's gradient */
+    int32_t  scaling;
+    double   base, factor, original_length, low_turns, high_turns;
+    float    magnitude;
+} aixk_rotary_spec;
+/* q, k: [batch, heads, sequence, head dim] of one element type and any two numbers of heads, k and k_out NULL for one tensor;
+ * positions: int32 [batch, sequence] in device memory (any view; negative ones turn back), read when the kernel runs.  Angles
+ * are exact to f32 at any position.  A result may be its operand itself (the same view): the turn is then in place. */
+int32_t aixk_rotary(aixk_ctx* ctx, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* positions, const aixk_rotary_spec* spec,
+                    const aixhip_tensor* q_out, const aixhip_tensor* k_out);
+
+/* A matrix product with what usually follows it: z = a . b + bias, out = act(z) + residual.  a [M, K] and b [K, N] are any 2-D
+ * views of one element type, bias [N] or [1, N], residual [M, N] any view (a broadcast one too); out and pre are dense [M, N].
+ * pre, if given, receives z rounded to the element type (what the backward pass needs); the activation is taken of z itself.
+ * out may be the residual itself (the same dense view).  GELU is the tanh form, 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))). */
+enum aixk_activation { AIXK_ACT_NONE = 0, AIXK_ACT_RELU = 1, AIXK_ACT_GELU = 2, AIXK_ACT_SILU = 3 };
+typedef struct aixk_epilogue {
+    const aixhip_tensor* bias;       /* or NULL */
+    const aixhip_tensor* residual;   /* or NULL */
+    const aixhip_tensor* pre;        /* or NULL */
+    int32_t activation;
+} aixk_epilogue;
+int32_t aixk_matmul_epilogue(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixk_epilogue* epilogue, const aixhip_tensor* out);
+/* Its gradients: dz = grad act'(pre), da = dz . b^T, db = a^T . dz, dbias = the sum of dz over its rows (f32, unrounded dz); the
+ * residual's gradient is grad itself.  grad, pre: [M, N] any views; dz: dense [M, N], the products read it rounded; da, db and
+ * dbias: dense, each may be NULL.  Without an activation dz = grad: pre and dz may then be NULL. */
+int32_t aixk_matmul_epilogue_backward(aixk_ctx* ctx, const aixhip_tensor* grad, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* pre,
+                                      int32_t activation, const aixhip_tensor* dz, const aixhip_tensor* da, const aixhip_tensor* db, const aixhip_tensor* dbias);
+
 /* ---- runtime-compiled fused elementwise kernels ------------------------- */
 /* Compile `source` (HIP C++, one extern "C" __global__ named `entry`) for gfx950 with hipRTC or
  * return the cached module for `key`.  *was_cached tells which.  Replaces the reference's

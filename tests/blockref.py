@@ -168,3 +168,93 @@ def T_float(x, dtype):
     if dtype == O.BF16:
         return (np.ascontiguousarray(x).astype(np.uint32) << 16).view(np.float32).astype(np.float64)
     return np.array(x, np.float64)
+
+
+# ---- rotary positions -----------------------------------------------------------------------------------------------
+
+def rotary(x, positions, dims, interleaved, inverse, frequencies, magnitude, dtype):
+    """x [b, h, s, d]; positions [b, s] -> the turned tensor and its bound: f32 sines and cosines, two products, one rounding."""
+    angle = positions.astype(np.float64)[:, None, :, None] * np.asarray(frequencies)
+    c, s = np.cos(angle) * magnitude, np.sin(angle) * magnitude * (-1 if inverse else 1)
+    i = np.arange(dims // 2)
+    first, second = (2 * i, 2 * i + 1) if interleaved else (i, i + dims // 2)
+    out, far = x.copy(), np.zeros_like(x)
+    out[..., first] = x[..., first] * c - x[..., second] * s
+    out[..., second] = x[..., first] * s + x[..., second] * c
+    # the fraction of a turn rounds to f32 (half a unit of at most half a turn: pi 2^-24), the functions are good to 2 units
+    mass = (np.abs(x[..., first]) + np.abs(x[..., second])) * magnitude * 10 * U32 + np.abs(angle) * 2.0 ** -50
+    far[..., first] = mass + HALF[dtype] * np.abs(out[..., first]) + TINY[dtype]
+    far[..., second] = mass + HALF[dtype] * np.abs(out[..., second]) + TINY[dtype]
+    return out, far
+
+
+def frequencies(dims, scaling="plain", base=10000.0, factor=1.0, original=1.0, low=0.0, high=1.0):
+    if scaling == "base" and dims > 2:
+        base = base * factor ** (dims / (dims - 2))
+    f = base ** (-2.0 * np.arange(dims // 2) / dims)
+    if scaling == "linear":
+        f = f / factor
+    if scaling == "parts":
+        kept = np.clip((original * f / (2 * math.pi) - low) / (high - low), 0, 1)
+        f = f * (kept + (1 - kept) / factor)
+    return f
+
+
+# ---- products with an epilogue --------------------------------------------------------------------------------------
+
+C_GELU = math.sqrt(2 / math.pi)
+
+
+def _argument(z, act):
+    return 2 * C_GELU * (z + 0.044715 * z ** 3) if act == "gelu" else z
+
+
+def activate(z, act):
+    """act(z), the size of its slope at most, and its own rounding: the exponent is good to a few units of itself."""
+    if act == "relu":
+        return np.maximum(z, 0), 1.0, 0 * z
+    if act == "none":
+        return z, 1.0, 0 * z
+    w = _argument(z, act)
+    y = z / (1 + np.exp(-np.clip(w, -700, 700)))
+    return y, 1.2, np.abs(y) * (np.minimum(np.abs(w), 80) + 8) * 6 * U32 + 1e-30
+
+
+def slope(z, act):
+    if act == "relu":
+        return (z > 0).astype(np.float64), 0 * z
+    if act == "none":
+        return np.ones_like(z), 0 * z
+    w = _argument(z, act)
+    e = np.exp(-np.clip(w, -700, 700))            # (the clip keeps e s at 1 on the far side and 0 on the near one)
+    s = 1 / (1 + e)
+    inner = 2 * C_GELU * (1 + 3 * 0.044715 * z ** 2) if act == "gelu" else 1.0
+    bend = z * s * (e * s) * inner
+    return s + bend, (np.minimum(np.abs(w), 80) + 8) * 6 * U32 * (s + np.abs(bend)) + 4 * U32
+
+
+def product_far(x, y, k):
+    """an f32 sum of k products; f32 operands go through the matrix unit as three bf16 planes, off by 2^-22 of a product"""
+    return ((k + 8) * U32 + 2.0 ** -22) * (np.abs(x) @ np.abs(y))
+
+
+def matmul_epilogue(a, b, bias, residual, act, dtype):
+    z = a @ b + (bias if bias is not None else 0)
+    z_far = product_far(a, b, a.shape[1]) + 2 * U32 * (np.abs(z) + np.abs(bias if bias is not None else 0))
+    y, steep, y_far = activate(z, act)
+    out = y + (residual if residual is not None else 0)
+    far = steep * z_far + y_far + 2 * U32 * (np.abs(y) + np.abs(out))
+    return out, far + HALF[dtype] * np.abs(out) + TINY[dtype], z, z_far + HALF[dtype] * np.abs(z) + TINY[dtype]
+
+
+def matmul_epilogue_backward(grad, a, b, pre, act, dtype):
+    s, s_far = slope(pre, act) if pre is not None else (np.ones_like(grad), 0 * grad)
+    dz = grad * s
+    exact_far = np.abs(grad) * s_far + U32 * np.abs(dz)
+    dz_far = exact_far + HALF[dtype] * np.abs(dz) + TINY[dtype]
+    m, n = grad.shape
+    da, db, dbias = dz @ b.T, a.T @ dz, dz.sum(0)
+    h, t = HALF[dtype], TINY[dtype]
+    return (dz, da, db, dbias), (dz_far, dz_far @ np.abs(b).T + product_far(dz, b.T, n) + h * np.abs(da) + t,
+                                 np.abs(a).T @ dz_far + product_far(a.T, dz, m) + h * np.abs(db) + t,
+                                 exact_far.sum(0) + (m + 8) * U32 * np.abs(dz).sum(0) + h * np.abs(dbias) + t)

@@ -82,3 +82,81 @@ def test_attention(backward):
         refused(lambda: call_attention({**good, **change}), message)
     if not backward:
         refused(lambda: call_attention({**good, "lse": None}), "null context")
+
+
+def ref(t):
+    return C.byref(t) if t is not None else None
+
+
+def ptr(t):
+    return C.pointer(t) if t is not None else None
+
+
+def call_rotary(d):
+    spec = K.RotarySpec(**{n: d[n] for n, _ in K.RotarySpec._fields_})
+    return LIB.aixk_rotary(None, ref(d["q"]), ref(d["k"]), ref(d["positions"]), C.byref(spec) if d["spec"] else None, ref(d["q_out"]), ref(d["k_out"]))
+
+
+def test_rotary():
+    at = At()
+    good = {"q": at(K.F16, 2, 4, 5, 64), "k": at(K.F16, 2, 1, 5, 64), "positions": at(K.I32, 2, 5), "q_out": at(K.F16, 2, 4, 5, 64), "k_out": at(K.F16, 2, 1, 5, 64),
+            "spec": True, "dims": 32, "interleaved": 0, "inverse": 0, "scaling": K.ROTARY_PARTS, "base": 1e4, "factor": 4.0, "original_length": 4096.0, "low_turns": 1.0,
+            "high_turns": 32.0, "magnitude": 1.0}
+    refused(lambda: call_rotary(good), "null context")
+    refused(lambda: call_rotary({**good, "k": None, "k_out": None}), "null context")
+    refused(lambda: call_rotary({**good, "q_out": good["q"], "k_out": good["k"]}), "null context")          # in place
+    nan, inf = float("nan"), float("inf")
+    for change, message in [
+        ({"spec": False}, "null spec"), ({"q": None}, "the queries"), ({"k": None}, "belong together"), ({"k_out": None}, "belong together"),
+        ({"q": at(K.F16, 4, 5, 64)}, "[batch, heads, sequence, head dim]"), ({"q": at(K.F64, 2, 4, 5, 64)}, "f32, f16 or bf16"),
+        ({"q_out": at(K.BF16, 2, 4, 5, 64)}, "bad descriptor"), ({"q_out": at(K.F16, 2, 5, 4, 64)}, "differs"), ({"k_out": at(K.F16, 2, 1, 5, 64, strides=(0, 0, 64, 1))}, "broadcast"),
+        ({"k": at(K.BF16, 2, 1, 5, 64), "k_out": at(K.BF16, 2, 1, 5, 64)}, "differ in type"), ({"k": at(K.F16, 2, 1, 6, 64), "k_out": at(K.F16, 2, 1, 6, 64)}, "sequence"),
+        ({"positions": None}, "int32"), ({"positions": at(K.I64, 2, 5)}, "int32"), ({"positions": at(K.I32, 5)}, "int32"), ({"positions": at(K.I32, 5, 2)}, "int32"),
+        ({"dims": 0}, "turned part"), ({"dims": 31}, "turned part"), ({"dims": 66}, "turned part"), ({"base": 0.0}, "positive"), ({"base": nan}, "positive"),
+        ({"magnitude": 0.0}, "positive"), ({"scaling": 4}, "unknown scaling"), ({"scaling": -1}, "unknown scaling"), ({"factor": 0.0}, "factor"), ({"factor": inf}, "factor"),
+        ({"original_length": 0.0}, "original length"), ({"low_turns": 32.0}, "high_turns"),
+        ({"q_out": good["k"]}, "bad descriptor"), ({"k_out": K.tensor(good["q"].data, K.F16, (2, 1, 5, 64))}, "overlaps"),
+        ({"q_out": K.tensor(good["q"].data, K.F16, (2, 4, 5, 64), offset=64)}, "overlaps"), ({"k_out": K.tensor(good["q_out"].data, K.F16, (2, 1, 5, 64))}, "share"),
+    ]:
+        refused(lambda: call_rotary({**good, **change}), message)
+
+
+def test_matmul_epilogue():
+    at = At()
+    good = {"a": at(K.BF16, 6, 8), "b": at(K.BF16, 8, 10), "bias": at(K.BF16, 10), "residual": at(K.BF16, 6, 10), "pre": at(K.BF16, 6, 10), "out": at(K.BF16, 6, 10), "act": 2, "spec": True}
+
+    def call(d):
+        spec = K.Epilogue(bias=ptr(d["bias"]), residual=ptr(d["residual"]), pre=ptr(d["pre"]), activation=d["act"])
+        return LIB.aixk_matmul_epilogue(None, ref(d["a"]), ref(d["b"]), C.byref(spec) if d["spec"] else None, ref(d["out"]))
+
+    for fine in ({}, {"bias": None, "residual": None, "pre": None}, {"bias": at(K.BF16, 1, 10)}, {"out": good["residual"]}, {"residual": at(K.BF16, 6, 10, strides=(0, 1))}):
+        refused(lambda: call({**good, **fine}), "null context")
+    for change, message in [
+        ({"spec": False}, "null epilogue"), ({"a": None}, "2-D"), ({"a": at(K.BF16, 1, 6, 8)}, "2-D"), ({"b": at(K.BF16, 9, 10)}, "inner dimensions"),
+        ({"b": at(K.F16, 8, 10)}, "one element type"), ({"a": at(K.I32, 6, 8), "b": at(K.I32, 8, 10)}, "one element type"), ({"a": at(K.F64, 6, 8), "b": at(K.F64, 8, 10)}, "one element type"),
+        ({"out": None}, "the result"), ({"out": at(K.F32, 6, 10)}, "the result"), ({"out": at(K.BF16, 6, 10, strides=(12, 1))}, "the result"), ({"out": at(K.BF16, 10, 6)}, "the result"),
+        ({"bias": at(K.F32, 10)}, "bias"), ({"bias": at(K.BF16, 6)}, "bias"), ({"bias": at(K.BF16, 10, 1)}, "bias"), ({"residual": at(K.BF16, 10)}, "residual"),
+        ({"pre": at(K.BF16, 6, 10, strides=(1, 6))}, "pre"), ({"act": 4}, "unknown activation"), ({"act": -1}, "unknown activation"),
+        ({"out": K.tensor(good["a"].data, K.BF16, (6, 10))}, "overlaps an operand"), ({"pre": good["out"]}, "pre overlaps"), ({"pre": good["residual"]}, "pre overlaps"),
+        ({"residual": K.tensor(good["out"].data, K.BF16, (6, 10), (0, 1))}, "overlaps the residual"), ({"bias": K.tensor(good["out"].data, K.BF16, (10,))}, "overlaps an operand"),
+    ]:
+        refused(lambda: call({**good, **change}), message)
+
+
+def test_matmul_epilogue_backward():
+    at = At()
+    good = {"grad": at(K.F32, 6, 10), "a": at(K.F32, 6, 8), "b": at(K.F32, 8, 10), "pre": at(K.F32, 6, 10), "act": 3, "dz": at(K.F32, 6, 10), "da": at(K.F32, 6, 8),
+            "db": at(K.F32, 8, 10), "dbias": at(K.F32, 10)}
+
+    def call(d):
+        return LIB.aixk_matmul_epilogue_backward(None, ref(d["grad"]), ref(d["a"]), ref(d["b"]), ref(d["pre"]), d["act"], ref(d["dz"]), ref(d["da"]), ref(d["db"]), ref(d["dbias"]))
+
+    for fine in ({}, {"da": None, "db": None, "dbias": None}, {"act": 0, "pre": None, "dz": None}, {"dbias": at(K.F32, 1, 10)}):
+        refused(lambda: call({**good, **fine}), "null context")
+    for change, message in [
+        ({"grad": None}, "grad"), ({"grad": at(K.F32, 10, 6)}, "grad"), ({"pre": None}, "needs pre and dz"), ({"dz": None}, "needs pre and dz"), ({"pre": at(K.F16, 6, 10)}, "pre"),
+        ({"dz": at(K.F32, 6, 10, strides=(1, 6))}, "dz"), ({"da": at(K.F32, 6, 10)}, "da"), ({"db": at(K.F32, 10, 8)}, "db"), ({"dbias": at(K.F32, 8)}, "dbias"),
+        ({"b": at(K.F32, 7, 10)}, "inner dimensions"), ({"act": 9}, "unknown activation"), ({"dz": good["grad"]}, "overlaps an operand"), ({"da": good["a"]}, "overlaps an operand"),
+        ({"dbias": K.tensor(good["dz"].data, K.F32, (10,))}, "results overlap"),
+    ]:
+        refused(lambda: call({**good, **change}), message)
