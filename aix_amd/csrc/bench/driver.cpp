@@ -284,4 +284,28 @@ int aixbench_transformer_captured(aixhip_device* handle, uint64_t layers, uint64
     });
 }
 
+// The transformer with its layers issued through the device's transformer-block operators: attention with `window` (0: none)
+// and `sinks`, `rotary_dims` elements of every head turned by their positions (0: none).  capture_at as above, < 0: every step
+// eagerly; graph_nodes may be NULL.
+int aixbench_transformer_blocks(aixhip_device* handle, uint64_t layers, uint64_t d_model, uint64_t heads, uint64_t seq, uint64_t batch, uint64_t vocab,
+                                int steps, uint64_t window, uint64_t sinks, uint64_t rotary_dims, int capture_at, const int32_t* tokens,
+                                const float* const* params, float* losses, float* grad_norms, double* step_seconds, uint64_t* graph_nodes)
+{
+    return guarded([&] {
+        DeviceHIP* dev = aix::hip::fromHandle(handle);
+        aixfe::TransformerConfig cfg{layers, d_model, heads, seq, batch, vocab, steps};
+        cfg.blocks = 1; cfg.window = window; cfg.sinks = sinks; cfg.rotaryDims = rotary_dims; cfg.captureAt = capture_at;
+        DeviceHIP::StepGraph* graph = nullptr;
+        const WideWindow window_(dev, capture_at >= 0);
+        aixfe::StepCapture capture;
+        capture.begin = [&] { dev->beginCapture(); };
+        capture.end = [&] { graph = dev->endCapture(); };
+        capture.replay = [&] { dev->replay(graph); };
+        try { aixfe::runTransformer(dev, cfg, tokens, params, losses, grad_norms, step_seconds, capture_at >= 0 ? &capture : nullptr); }
+        catch (...) { if (graph) dev->destroyGraph(graph); throw; }
+        if (graph_nodes) *graph_nodes = graph ? dev->graphNodes(graph) : 0;
+        if (graph) dev->destroyGraph(graph);
+    });
+}
+
 } // extern "C"

@@ -235,4 +235,73 @@ int32_t aixhip_memory_stats(aixhip_device* dev, uint64_t* live_bytes, uint64_t* 
     });
 }
 
+// ---- operators of transformer blocks
+namespace {
+// an optional operand
+struct Maybe {
+    DeviceTensorParams p;
+    bool on;
+    explicit Maybe(const aixhip_tensor* t) : on(t != nullptr) { if (t) p = P(t); }
+    const DeviceTensorParams* get() const { return on ? &p : nullptr; }
+};
+struct Attention {
+    Maybe lengths, starts;
+    aix::hip::AttentionSpec s;
+    explicit Attention(const aixk_attention_spec* spec) : lengths(spec ? spec->lengths : nullptr), starts(spec ? spec->starts : nullptr)
+    {
+        if (!spec) throw std::invalid_argument("null spec");
+        s.scale = spec->scale; s.causal = spec->causal != 0; s.window = spec->window; s.sinks = spec->sinks;
+        s.lengths = lengths.get(); s.starts = starts.get();
+    }
+};
+aix::hip::Activation activationOf(int32_t a)
+{
+    if (a < AIXK_ACT_NONE || a > AIXK_ACT_SILU) throw std::invalid_argument("unknown activation");
+    return static_cast<aix::hip::Activation>(a);
+}
+} // namespace
+
+int32_t aixhip_attention(aixhip_device* dev, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* v, const aixk_attention_spec* spec,
+                         const aixhip_tensor* result, const aixhip_tensor* lse)
+{
+    return guarded([&] { const Attention a(spec); const Maybe l(lse); D(dev).attention(P(q), P(k), P(v), a.s, P(result), l.get()); });
+}
+int32_t aixhip_attention_backward(aixhip_device* dev, const aixhip_tensor* grad, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* v,
+                                  const aixhip_tensor* out, const aixhip_tensor* lse, const aixk_attention_spec* spec,
+                                  const aixhip_tensor* dq, const aixhip_tensor* dk, const aixhip_tensor* dv)
+{
+    return guarded([&] { const Attention a(spec); D(dev).attentionBackward(P(grad), P(q), P(k), P(v), P(out), P(lse), a.s, P(dq), P(dk), P(dv)); });
+}
+int32_t aixhip_rotary(aixhip_device* dev, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* positions, const aixk_rotary_spec* spec,
+                      const aixhip_tensor* q_result, const aixhip_tensor* k_result)
+{
+    return guarded([&] {
+        if (!spec) throw std::invalid_argument("null spec");
+        if (spec->scaling < AIXK_ROTARY_PLAIN || spec->scaling > AIXK_ROTARY_PARTS) throw std::invalid_argument("unknown scaling");
+        const Maybe mk(k), mo(k_result);
+        aix::hip::RotarySpec s;
+        s.dims = spec->dims; s.interleaved = spec->interleaved != 0; s.inverse = spec->inverse != 0;
+        s.scaling = static_cast<aix::hip::RotaryScaling>(spec->scaling);
+        s.base = spec->base; s.factor = spec->factor; s.originalLength = spec->original_length; s.lowTurns = spec->low_turns; s.highTurns = spec->high_turns;
+        s.magnitude = spec->magnitude;
+        D(dev).rotary(P(q), mk.get(), P(positions), s, P(q_result), mo.get());
+    });
+}
+int32_t aixhip_matmul_epilogue(aixhip_device* dev, const aixhip_tensor* a, const aixhip_tensor* b, const aixk_epilogue* epilogue, const aixhip_tensor* result)
+{
+    return guarded([&] {
+        if (!epilogue) throw std::invalid_argument("null epilogue");
+        const Maybe bias(epilogue->bias), residual(epilogue->residual), pre(epilogue->pre);
+        D(dev).matmulEpilogue(P(a), P(b), {bias.get(), residual.get(), pre.get(), activationOf(epilogue->activation)}, P(result));
+    });
+}
+int32_t aixhip_matmul_epilogue_backward(aixhip_device* dev, const aixhip_tensor* grad, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* pre,
+                                        int32_t activation, const aixhip_tensor* dz, const aixhip_tensor* da, const aixhip_tensor* db, const aixhip_tensor* dbias)
+{
+    return guarded([&] {
+        const Maybe p(pre), z(dz), x(da), y(db), s(dbias);
+        D(dev).matmulEpilogueBackward(P(grad), P(a), P(b), p.get(), activationOf(activation), z.get(), x.get(), y.get(), s.get());
+    });
+}
+
 } // extern "C"

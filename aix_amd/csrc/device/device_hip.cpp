@@ -587,34 +587,41 @@ void DeviceHIP::flushFor(const void* a, const void* b, const void* c) { flushFor
 // it, which keeps the window -- and the kernels fused from it -- whole.
 void DeviceHIP::flushForOperands(const void* a, const void* b, const void* c, bool always)
 {
-    AIXHIP_TRACE("-- operator outside the planner (%zu recorded)", m_engine->pendingOps());
     const void* named[3] = {a, b, c};
-    const void* bases[3] = {nullptr, nullptr, nullptr};
     const int last = c ? 2 : b ? 1 : 0;
+    const bool writes[3] = {last == 0, last == 1, last == 2};
+    flushForMany(named, writes, 3, always);
+}
+
+// The same for any number of operands, each read or written.
+void DeviceHIP::flushForMany(const void* const* named, const bool* writes, size_t count, bool always)
+{
+    AIXHIP_TRACE("-- operator outside the planner (%zu recorded)", m_engine->pendingOps());
+    constexpr size_t kMost = 16;
+    if (count > kMost) throw std::logic_error("DeviceHIP: an operator with too many operands");
+    const void* bases[kMost] = {};
     bool dependent = always;
-    for (int k = 0; k < 3; ++k) {
+    for (size_t k = 0; k < count; ++k) {
         const void* p = named[k];
         if (!p) continue;
         const void* base = m_blocks.baseOf(p);              // an operand may point into the middle of a block
         if (base && base != p) { bases[k] = base; dependent = true; }
-        if (!dependent) dependent = k == last ? m_engine->pendingTouches(p) : m_engine->pendingWrites(p);
+        if (!dependent) dependent = writes[k] ? m_engine->pendingTouches(p) : m_engine->pendingWrites(p);
     }
-    markTouched(a);                                         // the caller is about to enqueue work on them
-    markTouched(b);
-    markTouched(c);
+    for (size_t k = 0; k < count; ++k) markTouched(named[k]);       // the caller is about to enqueue work on them
     auto& ex = *m_extras;
     auto meets = [&] {                                      // (every operand is asked about: all the groups in the way are marked)
         bool any = false;
         if (!ex.anyUses()) return any;
-        for (int k = 0; k < 3; ++k) {
-            if (k == last) { any = ex.meetsWrite(named[k]) || any; any = ex.meetsWrite(bases[k]) || any; }
+        for (size_t k = 0; k < count; ++k) {
+            if (writes[k]) { any = ex.meetsWrite(named[k]) || any; any = ex.meetsWrite(bases[k]) || any; }
             else           { any = ex.meetsRead(named[k]) || any;  any = ex.meetsRead(bases[k]) || any; }
         }
         return any;
     };
     if (meets()) issuePending(true);
     if (!dependent) return;
-    for (int k = 0; k < 3; ++k) {
+    for (size_t k = 0; k < count; ++k) {
         if (named[k]) m_engine->recordExternalRead(named[k]);
         if (bases[k]) m_engine->recordExternalRead(bases[k]);
     }
@@ -1815,6 +1822,131 @@ void DeviceHIP::indexAdd(const DeviceTensorParams& src, const DeviceTensorParams
     flushFor(src.data, indices.data, dst.data);
     aixhip_tensor ps, pd, pi; stagedPod(src, &ps, "indexAdd"); toPod(dst, &pd, "indexAdd"); stagedPod(indices, &pi, "indexAdd");
     check(aixk_index_add(m_ctx, &ps, &pd, &pi, dim));
+}
+
+// ---- operators of transformer blocks ------------------------------------------------------------
+// They run at once: what recorded and waiting work they depend on goes first, the rest stays in its window.
+struct DeviceHIP::BlockCall {
+    DeviceHIP* dev;
+    const char* op;
+    std::array<aixhip_tensor, 16> pods{};
+    std::array<const void*, 16> named{};
+    std::array<bool, 16> writes{};
+    size_t count{0};
+    BlockCall(DeviceHIP* d, const char* name) : dev(d), op(name) {}
+    // a result must be this device's memory; an operand in host memory is staged by ready()
+    void note(const DeviceTensorParams* p, bool write)
+    {
+        if (write && p) dev->requireDevice(*p, op);
+        named[count] = p ? p->data : nullptr;
+        writes[count] = write;
+        ++count;
+    }
+    void ready() { dev->flushForMany(named.data(), writes.data(), count, false); }
+    aixhip_tensor* pod(const DeviceTensorParams* p, size_t slot, bool write)
+    {
+        if (!p) return nullptr;
+        if (write) dev->toPod(*p, &pods[slot], op); else dev->stagedPod(*p, &pods[slot], op);
+        return &pods[slot];
+    }
+    // the kernel layer's workspaces are outside the pool: on ENOMEM the cached blocks go back to the driver, once
+    template <class F> void run(F&& f)
+    {
+        int status = f();
+        if (status == AIXK_ENOMEM && !dev->m_capturing) { dev->synchronize(); dev->emptyCache(); status = f(); }
+        dev->check(status);
+    }
+};
+
+void DeviceHIP::attention(const DeviceTensorParams& q, const DeviceTensorParams& k, const DeviceTensorParams& v, const AttentionSpec& spec,
+                          const DeviceTensorParams& result, const DeviceTensorParams* lse)
+{
+    const Marker marker_("attention");
+    AIXHIP_TRACE("attention %zu queries, %zu keys", q.size, k.size);
+    BlockCall c(this, "attention");
+    const DeviceTensorParams* in[] = {&q, &k, &v, spec.lengths, spec.starts};
+    for (const auto* p : in) c.note(p, false);
+    c.note(&result, true); c.note(lse, true);
+    c.ready();
+    aixhip_tensor* t[5];
+    for (size_t n = 0; n < 5; ++n) t[n] = c.pod(in[n], n, false);
+    const aixk_attention_spec s{spec.scale, spec.causal ? 1 : 0, spec.window, spec.sinks, t[3], t[4]};
+    const aixhip_tensor *o = c.pod(&result, 5, true), *l = c.pod(lse, 6, true);
+    c.run([&] { return aixk_attention(m_ctx, t[0], t[1], t[2], &s, o, l); });
+}
+
+void DeviceHIP::attentionBackward(const DeviceTensorParams& grad, const DeviceTensorParams& q, const DeviceTensorParams& k, const DeviceTensorParams& v,
+                                  const DeviceTensorParams& out, const DeviceTensorParams& lse, const AttentionSpec& spec,
+                                  const DeviceTensorParams& dq, const DeviceTensorParams& dk, const DeviceTensorParams& dv)
+{
+    const Marker marker_("attentionBackward");
+    AIXHIP_TRACE("attentionBackward %zu queries, %zu keys", q.size, k.size);
+    BlockCall c(this, "attentionBackward");
+    const DeviceTensorParams* in[] = {&grad, &q, &k, &v, &out, &lse, spec.lengths, spec.starts};
+    const DeviceTensorParams* to[] = {&dq, &dk, &dv};
+    for (const auto* p : in) c.note(p, false);
+    for (const auto* p : to) c.note(p, true);
+    c.ready();
+    aixhip_tensor *t[8], *r[3];
+    for (size_t n = 0; n < 8; ++n) t[n] = c.pod(in[n], n, false);
+    for (size_t n = 0; n < 3; ++n) r[n] = c.pod(to[n], 8 + n, true);
+    const aixk_attention_spec s{spec.scale, spec.causal ? 1 : 0, spec.window, spec.sinks, t[6], t[7]};
+    c.run([&] { return aixk_attention_backward(m_ctx, t[0], t[1], t[2], t[3], t[4], t[5], &s, r[0], r[1], r[2]); });
+}
+
+void DeviceHIP::rotary(const DeviceTensorParams& q, const DeviceTensorParams* k, const DeviceTensorParams& positions, const RotarySpec& spec,
+                       const DeviceTensorParams& qResult, const DeviceTensorParams* kResult)
+{
+    const Marker marker_("rotary");
+    AIXHIP_TRACE("rotary %zu + %zu elements", q.size, k ? k->size : size_t(0));
+    BlockCall c(this, "rotary");
+    const DeviceTensorParams* in[] = {&q, k, &positions};
+    for (const auto* p : in) c.note(p, false);
+    c.note(&qResult, true); c.note(kResult, true);
+    c.ready();
+    aixhip_tensor* t[3];
+    for (size_t n = 0; n < 3; ++n) t[n] = c.pod(in[n], n, false);
+    aixk_rotary_spec s{};
+    s.dims = (uint32_t)std::min<size_t>(spec.dims, 0xFFFFFFFFu);
+    s.interleaved = spec.interleaved; s.inverse = spec.inverse; s.scaling = (int32_t)spec.scaling;
+    s.base = spec.base; s.factor = spec.factor; s.original_length = spec.originalLength; s.low_turns = spec.lowTurns; s.high_turns = spec.highTurns;
+    s.magnitude = spec.magnitude;
+    const aixhip_tensor *oq = c.pod(&qResult, 3, true), *ok = c.pod(kResult, 4, true);
+    c.run([&] { return aixk_rotary(m_ctx, t[0], t[1], t[2], &s, oq, ok); });
+}
+
+void DeviceHIP::matmulEpilogue(const DeviceTensorParams& a, const DeviceTensorParams& b, const Epilogue& epilogue, const DeviceTensorParams& result)
+{
+    const Marker marker_("matmulEpilogue");
+    AIXHIP_TRACE("matmulEpilogue %zu x %zu elements", a.size, b.size);
+    BlockCall c(this, "matmulEpilogue");
+    const DeviceTensorParams* in[] = {&a, &b, epilogue.bias, epilogue.residual};
+    for (const auto* p : in) c.note(p, false);
+    c.note(epilogue.pre, true); c.note(&result, true);
+    c.ready();
+    aixhip_tensor* t[4];
+    for (size_t n = 0; n < 4; ++n) t[n] = c.pod(in[n], n, false);
+    const aixhip_tensor *pre = c.pod(epilogue.pre, 4, true), *o = c.pod(&result, 5, true);
+    const aixk_epilogue e{t[2], t[3], pre, (int32_t)epilogue.activation};
+    c.run([&] { return aixk_matmul_epilogue(m_ctx, t[0], t[1], &e, o); });
+}
+
+void DeviceHIP::matmulEpilogueBackward(const DeviceTensorParams& grad, const DeviceTensorParams& a, const DeviceTensorParams& b, const DeviceTensorParams* pre,
+                                       Activation activation, const DeviceTensorParams* dz, const DeviceTensorParams* da, const DeviceTensorParams* db,
+                                       const DeviceTensorParams* dbias)
+{
+    const Marker marker_("matmulEpilogueBackward");
+    AIXHIP_TRACE("matmulEpilogueBackward %zu x %zu elements", a.size, b.size);
+    BlockCall c(this, "matmulEpilogueBackward");
+    const DeviceTensorParams* in[] = {&grad, &a, &b, pre};
+    const DeviceTensorParams* to[] = {dz, da, db, dbias};
+    for (const auto* p : in) c.note(p, false);
+    for (const auto* p : to) c.note(p, true);
+    c.ready();
+    aixhip_tensor *t[4], *r[4];
+    for (size_t n = 0; n < 4; ++n) t[n] = c.pod(in[n], n, false);
+    for (size_t n = 0; n < 4; ++n) r[n] = c.pod(to[n], 4 + n, true);
+    c.run([&] { return aixk_matmul_epilogue_backward(m_ctx, t[0], t[1], t[2], t[3], (int32_t)activation, r[0], r[1], r[2], r[3]); });
 }
 
 } // namespace hip

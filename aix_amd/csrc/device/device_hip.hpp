@@ -23,6 +23,7 @@
 #pragma once
 
 #include "aix_compat.hpp"
+#include "block_operators.hpp"
 #include "fuse.hpp"
 
 #include <cstdint>
@@ -39,7 +40,7 @@ struct aixhip_device;
 
 namespace aix::hip {
 
-class DeviceHIP : public aix::Device {
+class DeviceHIP : public aix::Device, public BlockOperators {
 public:
     explicit DeviceHIP(size_t deviceIndex = 0);
     ~DeviceHIP() override;
@@ -93,6 +94,19 @@ public:
 
     void emptyCache() override;
     void synchronize() override;
+
+    // ---- operators of transformer blocks (block_operators.hpp): run at once, like matmul ----------------
+    void attention(const DeviceTensorParams& q, const DeviceTensorParams& k, const DeviceTensorParams& v, const AttentionSpec& spec,
+                   const DeviceTensorParams& result, const DeviceTensorParams* lse) override;
+    void attentionBackward(const DeviceTensorParams& grad, const DeviceTensorParams& q, const DeviceTensorParams& k, const DeviceTensorParams& v,
+                           const DeviceTensorParams& out, const DeviceTensorParams& lse, const AttentionSpec& spec,
+                           const DeviceTensorParams& dq, const DeviceTensorParams& dk, const DeviceTensorParams& dv) override;
+    void rotary(const DeviceTensorParams& q, const DeviceTensorParams* k, const DeviceTensorParams& positions, const RotarySpec& spec,
+                const DeviceTensorParams& qResult, const DeviceTensorParams* kResult) override;
+    void matmulEpilogue(const DeviceTensorParams& a, const DeviceTensorParams& b, const Epilogue& epilogue, const DeviceTensorParams& result) override;
+    void matmulEpilogueBackward(const DeviceTensorParams& grad, const DeviceTensorParams& a, const DeviceTensorParams& b, const DeviceTensorParams* pre,
+                                Activation activation, const DeviceTensorParams* dz, const DeviceTensorParams* da, const DeviceTensorParams* db,
+                                const DeviceTensorParams* dbias) override;
 
     // ---- beyond the interface -------------------------------------------------------------------
     // Explicit transfers for hosts that should not read device memory through the BAR mapping.
@@ -185,6 +199,8 @@ private:
     bool takeInit(const DeviceTensorParams& src, const DeviceTensorParams& dst, uint64_t* bits);
     void flushFor(const void* a = nullptr, const void* b = nullptr, const void* c = nullptr);
     void flushForOperands(const void* a, const void* b, const void* c, bool always);
+    void flushForMany(const void* const* named, const bool* writes, size_t count, bool always);
+    struct BlockCall;                                          // the operands of a transformer-block operator on their way to the kernel layer
     void flushWindow(bool final);
     bool fenceInterior(const void* a, const void* b = nullptr, const void* c = nullptr);   // true: flush again once the operator is recorded
     void emitFused(const aixhip::fuse::FusedSubgraphDescriptor& d);

@@ -536,8 +536,20 @@ public:
         return r;
     }
 
-private:
+    // The result of an operator with a backward function of its own: `fn` hands every input that wants one its seed;
+    // readsInputs as in Node::setBackward.
+    static Tensor fromOperator(Value v, const std::vector<Tensor>& inputs, std::function<void(Node*, const Value&)> fn, unsigned readsInputs)
+    {
+        bool anyGrad = false, anyNonLeaf = false;
+        std::vector<NodePtr> nodes;
+        for (const auto& t : inputs) { anyGrad |= t.isRequireGrad(); anyNonLeaf |= !t.m_node->isLeaf; nodes.push_back(t.m_node); }
+        Tensor r = makeResult(std::move(v), anyGrad, anyNonLeaf);
+        r.m_node->setBackward(std::move(nodes), std::move(fn), readsInputs);
+        return r;
+    }
     static bool wants(const NodePtr& n) { return n->requireGrad || n->retainGrad; }
+
+private:
 
     // aixCore.hpp:2017-2024
     static void defaultBackward(Node* n, const Value& seed)

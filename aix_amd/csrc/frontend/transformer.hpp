@@ -18,13 +18,20 @@
 // q, k, v are seen as [batch, heads, seq, d / heads] views (reshape + transpose, no copy), the
 // scores of all sequences and heads are one [batch, heads, seq, seq] tensor, and mask, softmax and
 // the product with v are one operator each over it.  The arithmetic per element is the same.
+//
+// blocks = 1 issues the layers through the device's transformer-block operators (blocks.hpp): projections with bias (and GELU,
+// and the residual) in the product's epilogue, optionally rotary positions, and attention as one operator, optionally with a
+// sliding window and leading keys that stay visible.  Without window and rotary positions it computes the same function
+// with fewer roundings on the way.
 #pragma once
 #include <functional>
 
+#include "blocks.hpp"
 #include "nn.hpp"
 
 #include <chrono>
 #include <cmath>
+#include <tuple>
 
 namespace aixfe {
 
@@ -33,6 +40,9 @@ struct TransformerConfig {
     int32_t steps;
     int32_t stackedAttention{0};
     int32_t captureAt{-1};        // >= 0 (and a StepCapture given): that step is captured, it and every later one is a replay
+    int32_t blocks{0};
+    uint64_t window{0}, sinks{0}; // of blocks' attention
+    uint64_t rotaryDims{0};       // of every head turned by its position (0: none)
 };
 
 
@@ -94,6 +104,10 @@ inline void runTransformer(Device* dev, const TransformerConfig& c, const int32_
     for (uint64_t i = 0; i < c.seq; ++i) for (uint64_t j = 0; j < c.seq; ++j) maskHost[i * c.seq + j] = j > i ? -30000.0f : 0.0f;
     const Tensor mask = Tensor(Value::fromHost(dev, F32, Shape{c.seq, c.seq}, maskHost.data()).to(BF16));
     const float scale = 1.0f / std::sqrt((float)dh);
+    const AttentionMask seen{scale, true, c.window, c.sinks, Value(), Value()};
+    aix::hip::RotarySpec turn;
+    turn.dims = c.rotaryDims;
+    const Value pos2 = pos.reshape(Shape{c.batch, c.seq});
     dev->synchronize();
 
     Tensor loss;                                                 // the captured step's graph of nodes: its tensors are what a replay writes
@@ -108,6 +122,17 @@ inline void runTransformer(Device* dev, const TransformerConfig& c, const int32_
         at = 2;
         for (uint64_t l = 0; l < c.layers; ++l, at += 16) {
             const Tensor h = layerNorm(x, P[at + 0], P[at + 1]);
+            if (c.blocks) {
+                const Shape split{c.batch, c.seq, c.heads, dh};
+                Tensor q4 = linear(h, W[at + 2], W[at + 3]).reshape(split).transpose(1, 2), k4 = linear(h, W[at + 4], W[at + 5]).reshape(split).transpose(1, 2);
+                const Tensor v4 = linear(h, W[at + 6], W[at + 7]).reshape(split).transpose(1, 2);
+                if (c.rotaryDims) std::tie(q4, k4) = rotary(q4, k4, pos2, turn);
+                const Tensor mixed = attention(q4, k4, v4, seen).transpose(1, 2).reshape(Shape{T, d});
+                x = linear(mixed, W[at + 8], W[at + 9], Activation::kNone, &x);
+                const Tensor inner = linear(layerNorm(x, P[at + 10], P[at + 11]), W[at + 12], W[at + 13], Activation::kGELU);
+                x = linear(inner, W[at + 14], W[at + 15], Activation::kNone, &x);
+                continue;
+            }
             const Tensor q = matmul(h, W[at + 2]) + W[at + 3];
             const Tensor k = matmul(h, W[at + 4]) + W[at + 5];
             const Tensor v = matmul(h, W[at + 6]) + W[at + 7];

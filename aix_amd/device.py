@@ -48,6 +48,11 @@ _SIGNATURES = {
     "aixhip_triu": [_P, _T, _T, C.c_int64],
     "aixhip_index_select": [_P, _T, _T, _T, C.c_size_t],
     "aixhip_index_add": [_P, _T, _T, _T, C.c_size_t],
+    "aixhip_attention": [_P, _T, _T, _T, C.POINTER(K.AttentionSpec), _T, _T],
+    "aixhip_attention_backward": [_P, _T, _T, _T, _T, _T, _T, C.POINTER(K.AttentionSpec), _T, _T, _T],
+    "aixhip_rotary": [_P, _T, _T, _T, C.POINTER(K.RotarySpec), _T, _T],
+    "aixhip_matmul_epilogue": [_P, _T, _T, C.POINTER(K.Epilogue), _T],
+    "aixhip_matmul_epilogue_backward": [_P, _T, _T, _T, _T, C.c_int32, _T, _T, _T, _T],
     "aixhip_empty_cache": [_P],
     "aixhip_synchronize": [_P],
     "aixhip_flush": [_P],

@@ -126,3 +126,22 @@ def transformer(dev, cfg, steps, data, stacked=False):
     run("aixbench_transformer", dev.handle, *cfg, steps, int(stacked), tokens.ctypes.data_as(C.POINTER(C.c_int32)), pp, losses.ctypes.data_as(_PF),
         norms.ctypes.data_as(_PF), secs.ctypes.data_as(C.POINTER(C.c_double)))
     return losses, norms, secs
+
+
+def transformer_blocks(dev, cfg, steps, data, window=0, sinks=0, rotary_dims=0, capture_at=-1):
+    """transformer() with the layers issued through the device's transformer-block operators: bias, GELU and residual in the
+    products' epilogues, attention as one operator with a sliding `window` (0: none) and `sinks` leading keys that stay
+    visible, `rotary_dims` elements of every head turned by their positions (0: none).  capture_at >= 0: that step is captured
+    into a HIP graph, it and all later ones are replays.  Returns (losses, gradient norms, seconds per step, graph nodes)."""
+    tokens, params = data
+    lib = load()
+    lib.aixbench_transformer_blocks.argtypes = [C.c_void_p] + [C.c_uint64] * 6 + [C.c_int] + [C.c_uint64] * 3 + [C.c_int, C.POINTER(C.c_int32), _PPF, _PF, _PF,
+                                                                                                                  C.POINTER(C.c_double), C.POINTER(C.c_uint64)]
+    losses = np.zeros(steps, np.float32)
+    norms = np.zeros((steps, len(params)), np.float32)
+    secs = np.zeros(steps, np.float64)
+    nodes = C.c_uint64(0)
+    pp = _pointer_array(params)
+    run("aixbench_transformer_blocks", dev.handle, *cfg, steps, window, sinks, rotary_dims, capture_at, tokens.ctypes.data_as(C.POINTER(C.c_int32)), pp,
+        losses.ctypes.data_as(_PF), norms.ctypes.data_as(_PF), secs.ctypes.data_as(C.POINTER(C.c_double)), C.byref(nodes))
+    return losses, norms, secs, int(nodes.value)

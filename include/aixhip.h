@@ -105,6 +105,20 @@ int32_t aixhip_index_add(aixhip_device* dev, const aixhip_tensor* src, const aix
 int32_t aixhip_empty_cache(aixhip_device* dev);
 int32_t aixhip_synchronize(aixhip_device* dev);
 
+/* ---- operators of transformer blocks, beyond aix::Device (the reference composes them from the operators above): the entry
+ * points of the same names in aixhip_kernels.h, which gives shapes, meanings and limits.  They run at once, after the recorded
+ * work they depend on; results must be this device's memory, operands may be host memory. */
+int32_t aixhip_attention(aixhip_device* dev, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* v, const aixk_attention_spec* spec,
+                         const aixhip_tensor* result, const aixhip_tensor* lse);
+int32_t aixhip_attention_backward(aixhip_device* dev, const aixhip_tensor* grad, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* v,
+                                  const aixhip_tensor* out, const aixhip_tensor* lse, const aixk_attention_spec* spec,
+                                  const aixhip_tensor* dq, const aixhip_tensor* dk, const aixhip_tensor* dv);
+int32_t aixhip_rotary(aixhip_device* dev, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* positions, const aixk_rotary_spec* spec,
+                      const aixhip_tensor* q_result, const aixhip_tensor* k_result);
+int32_t aixhip_matmul_epilogue(aixhip_device* dev, const aixhip_tensor* a, const aixhip_tensor* b, const aixk_epilogue* epilogue, const aixhip_tensor* result);
+int32_t aixhip_matmul_epilogue_backward(aixhip_device* dev, const aixhip_tensor* grad, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* pre,
+                                        int32_t activation, const aixhip_tensor* dz, const aixhip_tensor* da, const aixhip_tensor* db, const aixhip_tensor* dbias);
+
 /* ---- beyond aix::Device: what the reference exposes on its GPU device class for tests and tools ---- */
 /* Plan and enqueue what has been recorded, without waiting. */
 int32_t aixhip_flush(aixhip_device* dev);

@@ -104,6 +104,13 @@ int32_t aixk_matmul(aixk_ctx* c, const aixhip_tensor*, const aixhip_tensor*, con
     ++c->launches; c->log += "aixk_matmul;";
     return AIXK_OK;
 }
+STUB_OP(aixk_attention, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixk_attention_spec*, const aixhip_tensor*, const aixhip_tensor*)
+STUB_OP(aixk_attention_backward, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*,
+        const aixk_attention_spec*, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*)
+STUB_OP(aixk_rotary, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixk_rotary_spec*, const aixhip_tensor*, const aixhip_tensor*)
+STUB_OP(aixk_matmul_epilogue, const aixhip_tensor*, const aixhip_tensor*, const aixk_epilogue*, const aixhip_tensor*)
+STUB_OP(aixk_matmul_epilogue_backward, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, int32_t, const aixhip_tensor*,
+        const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*)
 STUB_OP(aixk_matmul_batched, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*)
 int32_t aixk_matmul_grouped(aixk_ctx* c, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, uint32_t count)
 {
