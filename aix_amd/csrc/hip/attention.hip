@@ -31,7 +31,7 @@ struct ForwardArgs {
 // keeps exp in range gives the same quotient), so the accumulators are rarely rescaled.  P is rounded to the operands'
 // type for the second product, as the matrix unit takes it; the sum is taken from the f32 values.
 template <class T, int DP>
-__global__ __launch_bounds__(256) void attention_k(ForwardArgs a)
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(ForwardArgs a)
 {
     typedef Mma<T> M;
     typedef typename M::Frag Frag;
@@ -69,6 +69,7 @@ __global__ __launch_bounds__(256) void attention_k(ForwardArgs a)
     float m = -__builtin_inff(), l = 0.0f;                    // m in units of log2, l this half's part of the sum
     const float c2 = s.scale * kLog2e;
 
+    const Keys seen = keys_of(s, r.length, p);
     const Tiles t = tiles_of(s, r.length, r.start + i0, r.start + i1, KT);
     Stage<T, DP, KT, 256> sk, sv;
     if (t.n) {
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(256) void attention_k(ForwardArgs a)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
                     const i32 j = j0 + kb * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
-                    x[kb][v] = visible(s, r.length, p, j) ? x[kb][v] : -__builtin_inff();
+                    x[kb][v] = seen(j) ? x[kb][v] : -__builtin_inff();
                 }
         }
         float top = x[0][0];
@@ -212,6 +213,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs 
     const float c2 = s.scale * kLog2e;
 
     // this workgroup's share of the visible steps; its waves take them in turn
+    const Keys seen = keys_of(s, r.length, p);
     const Tiles t = tiles_of(s, r.length, p0, p1, KT);
     const i32 from = (i32)((u64)(u32)t.n * split / a.splits), to = (i32)((u64)(u32)t.n * (split + 1) / a.splits);
 
@@ -271,7 +273,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs 
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                x[kb][v] = visible(s, r.length, p, j0 + kb * 16 + 4 * g + v) ? x[kb][v] * c2 : -__builtin_inff();
+                x[kb][v] = seen(j0 + kb * 16 + 4 * g + v) ? x[kb][v] * c2 : -__builtin_inff();
                 top = fmaxf(top, x[kb][v]);
             }
         top = fmaxf(top, __shfl_xor(top, 16, 64));

@@ -52,10 +52,39 @@ __device__ __forceinline__ Row row_of(const Shape& s, u32 b)
     return r;
 }
 
-__device__ __forceinline__ bool visible(const Shape& s, i32 length, i32 p, i32 j)
+// The keys the query at position p sees: lo <= j < lo + n, and j < sink.  Three comparisons per key without a branch (the mask's
+// definition written out per element becomes a branch per condition and element).
+struct Keys {
+    i32 lo; u32 n; i32 sink;
+    __device__ __forceinline__ bool operator()(i32 j) const { return ((u32)(j - lo) < n) | (j < sink); }
+};
+__device__ __forceinline__ Keys keys_of(const Shape& s, i32 length, i32 p)
 {
-    const i32 away = p > j ? p - j : j - p;
-    return j < length && p >= 0 && (!s.causal || j <= p) && (!s.window || away < s.window || j < s.sinks);
+    i32 hi = length, lo = 0;                                  // [lo, hi)
+    if (s.causal && p + 1 < hi) hi = p + 1;
+    Keys k{0, 0u, 0};
+    if (p < 0) return k;
+    if (s.window) {
+        k.sink = s.sinks < hi ? s.sinks : hi;
+        if ((i64)p + s.window < hi) hi = p + s.window;
+        if (p >= s.window) lo = p - s.window + 1;
+    }
+    k.lo = lo;
+    k.n = hi > lo ? (u32)(hi - lo) : 0u;
+    return k;
+}
+// The positions that see key j, lo <= p < lo + n.
+struct Queries {
+    i32 lo; u32 n;
+    __device__ __forceinline__ bool operator()(i32 p) const { return (u32)(p - lo) < n; }
+};
+__device__ __forceinline__ Queries queries_of(const Shape& s, i32 length, i32 j)
+{
+    if (j >= length) return Queries{0, 0u};
+    const bool near = s.window && j >= s.sinks;
+    const i32 lo = s.causal ? j : near && j >= s.window ? j - s.window + 1 : 0;
+    const i64 hi = near && (i64)j + s.window < 0x7FFFFFFF ? (i64)j + s.window : 0x7FFFFFFF;
+    return Queries{lo, (u32)(hi - lo)};
 }
 // every / no pair of the rows at positions [p0, p1] and the keys [j0, j1] is visible
 __device__ __forceinline__ bool all_visible(const Shape& s, i32 length, i32 p0, i32 p1, i32 j0, i32 j1)
@@ -162,6 +191,11 @@ template <class T> __device__ __forceinline__ typename Mma<T>::Frag load8(const 
     }
     return f;
 }
+
+// Waves per SIMD a kernel is compiled for: two where a wave's share of the 512 registers then holds its accumulators, fragments
+// and staged words (rows of up to 256 bytes), else one.  Two waves cover each other's exponentials, barriers and LDS reads:
+// 8192 queries, window 2048, head dim 128 in bf16 510 -> WAVES_A us.
+template <class T, int DP> constexpr int waves_per_simd() { return DP * (int)sizeof(T) <= 256 ? 2 : 1; }
 
 // ---- a tile of ROWS x DP elements in LDS --------------------------------------------------------------------------------
 // 16-byte word c of row r is kept in slot c ^ turn(r).  Reading one word from each of 16 consecutive rows then touches all

@@ -28,7 +28,7 @@ struct BackwardArgs {
 
 // As in attention_k the scores are transposed (a lane = one query): dS^T, rounded, feeds dq^T = K^T dS^T as it lies.
 template <class T, int DP, int KT>
-__global__ __launch_bounds__(256) void attention_dq_k(BackwardArgs a)
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k(BackwardArgs a)
 {
     typedef Mma<T> M;
     typedef typename M::Frag Frag;
@@ -81,6 +81,7 @@ __global__ __launch_bounds__(256) void attention_dq_k(BackwardArgs a)
     for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
     const float c2 = s.scale * kLog2e;
 
+    const Keys seen = keys_of(s, r.length, p);
     const Tiles t = tiles_of(s, r.length, r.start + i0, r.start + i1, KT);
     Stage<T, DP, KT, 256> sk, sv;
     if (t.n) {
@@ -114,9 +115,11 @@ __global__ __launch_bounds__(256) void attention_dq_k(BackwardArgs a)
             float e[16];
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-                float w = exp2_of(x[v] * c2 - lse2) * (dp[v] - delta);
-                if (masked && !visible(s, r.length, p, k0 + 8 * (v >> 2) + 4 * half + (v & 3))) w = 0.0f;
-                e[v] = w;
+                e[v] = exp2_of(x[v] * c2 - lse2) * (dp[v] - delta);
+            }
+            if (masked) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) e[v] = seen(k0 + 8 * (v >> 2) + 4 * half + (v & 3)) ? e[v] : 0.0f;
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -135,10 +138,16 @@ __global__ __launch_bounds__(256) void attention_dq_k(BackwardArgs a)
             put4<T>(row, a.dq.d, a.whole_dq, d * 32 + g * 8 + half * 4, s.D, acc[d][4 * g] * s.scale, acc[d][4 * g + 1] * s.scale, acc[d][4 * g + 2] * s.scale, acc[d][4 * g + 3] * s.scale);
 }
 
-// A wave keeps 32 keys and values in registers; the queries and gradients of every head of the group come by in tiles of QT
-// rows.  Here a lane is one key: P and dS, rounded, feed dv^T = grad^T P and dk^T = q^T dS as they lie.
+// A wave keeps 32 keys, its 32 values (in LDS where a row is 256 bytes or more: the registers then hold two waves per SIMD) and
+// both sums; the queries and gradients of every head of the group come by in tiles of QT rows.  Here a lane is one key: P and
+// dS, rounded, feed dv^T = grad^T P and dk^T = q^T dS as they lie.
+template <class T, int DP> struct KeyBlock {
+    static constexpr bool kValuesInLds = DP * sizeof(T) >= 256 && DP * sizeof(T) <= 512;
+    static constexpr int kRows = DP * sizeof(T) <= 128 ? 64 : 32;                      // QT
+    static constexpr size_t kLds = 2 * (size_t)kRows * DP * sizeof(T) + 2 * kRows * sizeof(float) + (kValuesInLds ? 128 * DP * sizeof(T) : 0);
+};
 template <class T, int DP, int QT>
-__global__ __launch_bounds__(256) void attention_dkdv_k(BackwardArgs a)
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dkdv_k(BackwardArgs a)
 {
     typedef Mma<T> M;
     typedef typename M::Frag Frag;
@@ -149,6 +158,8 @@ __global__ __launch_bounds__(256) void attention_dkdv_k(BackwardArgs a)
     char* gs = lds + QT * L::PITCH;
     float* ls = (float*)(lds + 2 * QT * L::PITCH);            // lse (log2), delta of the tile's rows
     float* ds = ls + QT;
+    constexpr bool VL = KeyBlock<T, DP>::kValuesInLds;
+    char* vs = (char*)(ds + QT);                              // the values of all 128 keys, if they are kept here
     const Shape& s = a.s;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -161,14 +172,28 @@ __global__ __launch_bounds__(256) void attention_dkdv_k(BackwardArgs a)
     const i32 j0 = k0 + wave * 32, j = j0 + (lane & 31);
     const bool on = j < r.length;
 
-    Frag kf[DC], vf[DC];
+    Frag kf[DC], vf[VL ? 1 : DC];
     {
         const u64 row = (u64)(u32)(on ? j : 0);
         const T* rk = (const T*)a.k.p + b * a.k.b + hk * a.k.h + row * a.k.s;
         const T* rv = (const T*)a.v.p + b * a.v.b + hk * a.v.h + row * a.v.s;
 #pragma unroll
-        for (int c = 0; c < DC; ++c) { kf[c] = load8<T>(rk, c * 16 + half * 8, s.DW, on); vf[c] = load8<T>(rv, c * 16 + half * 8, s.DW, on); }
+        for (int c = 0; c < DC; ++c) {
+            kf[c] = load8<T>(rk, c * 16 + half * 8, s.DW, on);
+            if constexpr (!VL) vf[c] = load8<T>(rv, c * 16 + half * 8, s.DW, on);
+        }
     }
+    if constexpr (VL) {                                       // (each wave reads its own rows only, but the loop's first barrier comes in between anyway)
+        if (k0 <= k1) {
+            Stage<T, DP, 128, 256> sv;
+            sv.load((const T*)a.v.p + b * a.v.b + hk * a.v.h, a.v.s, k0, r.length, s.DW, tid);
+            sv.store(vs, k0, r.length, s.DW, tid);
+        }
+    }
+    auto value = [&](int c) {
+        if constexpr (VL) return L::row(vs, wave * 32 + (lane & 31), 2 * c + half);
+        else return vf[c];
+    };
     f32x16 dk[DB], dv[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) { dk[d] = f32x16{}; dv[d] = f32x16{}; }
@@ -185,34 +210,39 @@ __global__ __launch_bounds__(256) void attention_dkdv_k(BackwardArgs a)
         if (lo < r.start) lo = r.start;
         if (lo < hi) { i_lo = (i32)(lo - r.start); i_hi = (i32)(hi - r.start); }
     }
+    const Queries seen = queries_of(s, r.length, j);
     const i32 first = i_lo / QT, per = i_lo < i_hi ? (i_hi + QT - 1) / QT - first : 0;
     const u64 total = (u64)(u32)per * s.G;
     const u64 from = total * split / a.splits, to = total * (split + 1) / a.splits;
 
+    // the (head of the group, tile) of a step, stepped on by counting (a division per step costs more than its products)
+    struct At { u32 g; i32 tile; };
+    auto on_from = [&](At& at) { if (++at.tile == per) { at.tile = 0; ++at.g; } };
     Stage<T, DP, QT, 256> sq, sg;
     float next_l = 0.0f, next_d = 0.0f;
-    auto load = [&](u64 n) {
-        const u32 h = hk * s.G + (u32)(n / (u32)per);
-        const i32 i0 = (first + (i32)(n % (u32)per)) * QT;
+    auto load = [&](const At& at) {
+        const u32 h = hk * s.G + at.g;
+        const i32 i0 = (first + at.tile) * QT;
         sq.load((const T*)a.q.p + b * a.q.b + h * a.q.h, a.q.s, i0, s.SQ, s.DW, tid);
         sg.load((const T*)a.grad.p + b * a.grad.b + h * a.grad.h, a.grad.s, i0, s.SQ, s.DW, tid);
         if (tid < QT) {
             const i32 i = i0 + tid < s.SQ ? i0 + tid : s.SQ - 1;
-            const u64 at = ((u64)b * s.H + h) * (u64)(u32)s.SQ + (u32)i;
-            const float saved = a.lse[at];
-            next_l = i0 + tid < s.SQ && saved != -__builtin_inff() ? saved * kLog2e : __builtin_inff();
-            next_d = a.delta[at];
+            const u64 row = ((u64)b * s.H + h) * (u64)(u32)s.SQ + (u32)i;
+            next_l = a.lse[row];                               // (looked at when it is stored: here it would wait for every load in flight)
+            next_d = a.delta[row];
         }
     };
-    if (from < to) load(from);
-    for (u64 n = from; n < to; ++n) {
-        const i32 i0 = (first + (i32)(n % (u32)per)) * QT;
+    At now{0, 0};
+    if (from < to) { now.g = (u32)(from / (u32)per); now.tile = (i32)(from % (u32)per); load(now); }
+    At next = now;
+    for (u64 n = from; n < to; ++n, now = next) {
+        const i32 i0 = (first + now.tile) * QT;
         __syncthreads();
         sq.store(qs, i0, s.SQ, s.DW, tid);
         sg.store(gs, i0, s.SQ, s.DW, tid);
-        if (tid < QT) { ls[tid] = next_l; ds[tid] = next_d; }
+        if (tid < QT) { ls[tid] = i0 + tid < s.SQ && next_l != -__builtin_inff() ? next_l * kLog2e : __builtin_inff(); ds[tid] = next_d; }
         __syncthreads();
-        if (n + 1 < to) load(n + 1);
+        if (n + 1 < to) { on_from(next); load(next); }
 #pragma unroll
         for (int qb = 0; qb < QT / 32; ++qb) {
             const i32 q0 = i0 + qb * 32, q1 = q0 + 31 < s.SQ ? q0 + 31 : s.SQ - 1;
@@ -221,7 +251,7 @@ __global__ __launch_bounds__(256) void attention_dkdv_k(BackwardArgs a)
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
                 x = M::run32(L::row(qs, qb * 32 + (lane & 31), 2 * c + half), kf[c], x);
-                dp = M::run32(L::row(gs, qb * 32 + (lane & 31), 2 * c + half), vf[c], dp);
+                dp = M::run32(L::row(gs, qb * 32 + (lane & 31), 2 * c + half), value(c), dp);
             }
             const bool masked = !all_visible(s, r.length, r.start + q0, r.start + q1, j0, j0 + 31);
             float e[16], w[16];
@@ -230,11 +260,16 @@ __global__ __launch_bounds__(256) void attention_dkdv_k(BackwardArgs a)
                 const f32x4 l4 = *(const f32x4*)(ls + qb * 32 + g * 8 + half * 4), d4 = *(const f32x4*)(ds + qb * 32 + g * 8 + half * 4);
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
-                    float y = exp2_of(x[4 * g + v] * c2 - l4[v]);
-                    float z = y * (dp[4 * g + v] - d4[v]);
-                    if (masked && !visible(s, r.length, r.start + q0 + 8 * g + 4 * half + v, j)) y = z = 0.0f;
-                    e[4 * g + v] = y;
-                    w[4 * g + v] = z;
+                    e[4 * g + v] = exp2_of(x[4 * g + v] * c2 - l4[v]);
+                    w[4 * g + v] = e[4 * g + v] * (dp[4 * g + v] - d4[v]);
+                }
+            }
+            if (masked) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const bool ok = seen(r.start + q0 + 8 * (v >> 2) + 4 * half + (v & 3));
+                    e[v] = ok ? e[v] : 0.0f;
+                    w[v] = ok ? w[v] : 0.0f;
                 }
             }
 #pragma unroll
@@ -324,9 +359,10 @@ template <class T, int DP> int backward(aixk_ctx* ctx, const Call& c, BackwardAr
         AIXK_TRY(block_scratch(ctx, kScratchParts, (size_t)splits * 2 * rows * DP * sizeof(float), &ws));
         a.part = (float*)ws;
     }
-    constexpr size_t lds = 2 * (size_t)KT * DP * sizeof(T) + 2 * KT * sizeof(float);
-    AIXK_TRY(allow_lds(attention_dkdv_k<T, DP, KT>, lds));
-    hipLaunchKernelGGL((attention_dkdv_k<T, DP, KT>), dim3((unsigned)(grid * splits)), dim3(256), lds, ctx->stream, a);
+    constexpr int QT = KeyBlock<T, DP>::kRows;
+    constexpr size_t lds = KeyBlock<T, DP>::kLds;
+    AIXK_TRY(allow_lds(attention_dkdv_k<T, DP, QT>, lds));
+    hipLaunchKernelGGL((attention_dkdv_k<T, DP, QT>), dim3((unsigned)(grid * splits)), dim3(256), lds, ctx->stream, a);
     AIXK_HIP(hipGetLastError());
     if (splits > 1) {
         constexpr u32 per = 256 / (DP / 4);
