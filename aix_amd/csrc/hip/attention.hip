@@ -150,6 +150,121 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
             put4<T>(row, a.out.d, a.whole, d * 32 + g * 8 + half * 4, s.D, o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
 }
 
+// The same on 16 queries per wave, 64 per workgroup, with v_mfma 16x16: for f32, whose matrix instructions are a sixteenth as
+// fast (a wave of 32 queries takes 7 us for a tile of 64 keys: half the queries are twice the waves to fill the chip with, and
+// the head dim's tail is left out), and for grids of 128-query workgroups that leave compute units without one.
+template <class T, int DP>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention16_k(ForwardArgs a)
+{
+    typedef Mma<T> M;
+    typedef typename M::Frag Frag;
+    typedef Tile<T, DP> L;
+    constexpr int KT = DP * sizeof(T) <= 512 ? 64 : 32, SUB = KT / 16, DB = DP / 16, DC = DP / 32;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char* ks = lds;
+    char* vs = lds + KT * L::PITCH;
+    const Shape& s = a.s;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c15 = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    const u32 id = xcd_order(blockIdx.x, gridDim.x);
+    const u32 head = id / a.tiles, tile = a.tiles - 1 - id % a.tiles;
+    const u32 b = head / s.H, h = head % s.H, hk = h / s.G;
+    const Row r = row_of(s, b);
+    const T* K = (const T*)a.k.p + b * a.k.b + hk * a.k.h;
+    const T* V = (const T*)a.v.p + b * a.v.b + hk * a.v.h;
+    const i32 i0 = (i32)tile * 64, i1 = i0 + 63 < s.SQ ? i0 + 63 : s.SQ - 1;
+    const i32 w0 = i0 + wave * 16, w1 = w0 + 15 < s.SQ ? w0 + 15 : s.SQ - 1;
+    const i32 i = w0 + c15, p = r.start + i;
+    const bool on = i < s.SQ;
+
+    Frag q[DC];
+    {
+        const T* row = (const T*)a.q.p + b * a.q.b + h * a.q.h + (u64)(on ? i : 0) * a.q.s;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) q[c] = load8<T>(row, c * 32 + g * 8, s.DW, on);
+    }
+    f32x4 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x4{};
+    float m = -__builtin_inff(), l = 0.0f;
+    const float c2 = s.scale * kLog2e;
+
+    const Keys seen = keys_of(s, r.length, p);
+    const Tiles t = tiles_of(s, r.length, r.start + i0, r.start + i1, KT);
+    Stage<T, DP, KT, 256> sk, sv;
+    if (t.n) {
+        const i32 j0 = tile_at(t, 0) * KT;
+        sk.load(K, a.k.s, j0, r.length, s.DW, tid);
+        sv.load(V, a.v.s, j0, r.length, s.DW, tid);
+    }
+    for (i32 n = 0; n < t.n; ++n) {
+        const i32 j0 = tile_at(t, n) * KT;
+        __syncthreads();
+        sk.store(ks, j0, r.length, s.DW, tid);
+        sv.store(vs, j0, r.length, s.DW, tid);
+        __syncthreads();
+        if (n + 1 < t.n) {
+            const i32 next = tile_at(t, n + 1) * KT;
+            sk.load(K, a.k.s, next, r.length, s.DW, tid);
+            sv.load(V, a.v.s, next, r.length, s.DW, tid);
+        }
+        if (w0 > w1 || none_visible(s, r.length, r.start + w0, r.start + w1, j0, j0 + KT - 1)) continue;
+
+        f32x4 x[SUB];
+#pragma unroll
+        for (int k = 0; k < SUB; ++k) x[k] = f32x4{};
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+            if (past<T>(c * 32, s.DW)) break;
+#pragma unroll
+            for (int k = 0; k < SUB; ++k) x[k] = M::run16(L::row(ks, k * 16 + c15, 4 * c + g), q[c], x[k]);
+        }
+        const bool masked = !all_visible(s, r.length, r.start + w0, r.start + w1, j0, j0 + KT - 1);
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int k = 0; k < SUB; ++k)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                if (masked) x[k][v] = seen(j0 + k * 16 + 4 * g + v) ? x[k][v] : -__builtin_inff();
+                top = fmaxf(top, x[k][v]);
+            }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * c2;
+        if (__any(top > m + 8.0f)) {
+            const float raised = fmaxf(m, top);
+            const float keep = raised == -__builtin_inff() ? 0.0f : exp2_of(m - raised);
+            m = raised;
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) o[d][v] *= keep;
+        }
+        const float ref = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+        for (int k = 0; k < SUB / 2; ++k) {
+            float e[8];
+#pragma unroll
+            for (int v = 0; v < 8; ++v) { e[v] = exp2_of(x[2 * k + (v >> 2)][v & 3] * c2 - ref); l += e[v]; }
+            const Frag w = M::pack8(e);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                if (past<T>(d * 16, s.DW)) break;
+                o[d] = M::run16(L::column16(vs, k * 32, d, lane), w, o[d]);
+            }
+        }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (!on) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (a.lse && g == 0) a.lse[((u64)b * s.H + h) * (u64)s.SQ + (u32)i] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * kLn2;
+    char* row = a.out.p + (b * a.out.b + h * a.out.h + (u64)(u32)i * a.out.s) * sizeof(T);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) put4<T>(row, a.out.d, a.whole, d * 16 + g * 4, s.D, o[d].x * inv, o[d].y * inv, o[d].z * inv, o[d].w * inv);
+}
+
 // ---- few queries ----------------------------------------------------------------------------------------------------------
 
 struct SplitArgs {
@@ -424,13 +539,25 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
     const u64 wide = (u64)s.B * s.H * (((u32)s.SQ + 127) / 128), narrow = (u64)s.B * s.HK * ((R + 15) / 16);
     // Few queries: at most 32 rows per key head.
     if (R > 32) {
+        if (sizeof(T) == 4 || wide < (u64)ctx->cus) {
+            const u64 grid = (u64)s.B * s.H * (((u32)s.SQ + 63) / 64);
+            AIXK_REQUIRE(grid < (1ull << 31), "attention: too many rows");
+            ForwardArgs a{s, c.q, c.k, c.v, c.out, c.lse, ((u32)s.SQ + 63) / 64, c.whole_out};
+            constexpr size_t lds = 2 * (DP * sizeof(T) <= 512 ? 64 : 32) * DP * sizeof(T);
+            AIXK_TRY(allow_lds(attention16_k<T, DP>, lds));
+            hipLaunchKernelGGL((attention16_k<T, DP>), dim3((unsigned)grid), dim3(256), lds, ctx->stream, a);
+            AIXK_HIP(hipGetLastError());
+            return AIXK_OK;
+        }
         AIXK_REQUIRE(wide < (1ull << 31), "attention: too many rows");
+        if constexpr (sizeof(T) == 2) {
         ForwardArgs a{s, c.q, c.k, c.v, c.out, c.lse, ((u32)s.SQ + 127) / 128, c.whole_out};
         constexpr size_t lds = 2 * 64 * DP * sizeof(T);
         AIXK_TRY(allow_lds(attention_k<T, DP>, lds));
         hipLaunchKernelGGL((attention_k<T, DP>), dim3((unsigned)wide), dim3(256), lds, ctx->stream, a);
         AIXK_HIP(hipGetLastError());
         return AIXK_OK;
+        }
     }
     SplitArgs a{s, c.q, c.k, c.v, c.out, c.lse, (R + 15) / 16, 1, c.whole_out, nullptr, nullptr};
     // Shares of the keys until every compute unit has four workgroups, but no share below one step of all waves.  What a row

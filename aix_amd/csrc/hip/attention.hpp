@@ -192,6 +192,10 @@ template <class T> __device__ __forceinline__ typename Mma<T>::Frag load8(const 
     return f;
 }
 
+// Elements from d on lie past the head dim and their products are left out: f32, whose matrix instructions take 16 times as
+// long as the branch's; the 16-bit kernels multiply the zeros, which keeps their loops free of branches.
+template <class T> __device__ __forceinline__ bool past(int d, u32 DW) { return sizeof(T) == 4 && d >= (int)DW; }
+
 // Waves per SIMD a kernel is compiled for: two where a wave's share of the 512 registers then holds its accumulators, fragments
 // and staged words (rows of up to 256 bytes), else one.  Two waves cover each other's exponentials, barriers and LDS reads:
 // 8192 queries, window 2048, head dim 128 in bf16 510 -> WAVES_A us.
@@ -232,6 +236,25 @@ template <class T, int DP> struct Tile {
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = *(const float*)(lds + at(r0 + 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3), c >> 2) + 4 * (c & 3));
+            return Mma<T>::pack8(x);
+        }
+    }
+    // the same for 16 x 16 accumulators: column 16 block + lane % 16, the rows r0 + 16 (j / 4) + 4 (lane / 16) + j % 4
+    static __device__ __forceinline__ typename Mma<T>::Frag column16(const char* lds, int r0, int block, int lane)
+    {
+        const int g = lane >> 4, i = lane & 15;
+        if constexpr (sizeof(T) == 2) {
+            const int r = r0 + 4 * g + (i >> 2), word = 2 * block + ((i & 3) >> 1);
+            const char* lo = lds + at(r, word) + 8 * (i & 1);
+            const char* hi = lds + at(r + 16, word) + 8 * (i & 1);
+            const u32x2 l = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lo));
+            const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi));
+            return u32x4{l.x, l.y, h.x, h.y};
+        } else {
+            const int c = 16 * block + i;
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = *(const float*)(lds + at(r0 + 16 * (j >> 2) + 4 * g + (j & 3), c >> 2) + 4 * (c & 3));
             return Mma<T>::pack8(x);
         }
     }

@@ -9,6 +9,8 @@
 #include "attention.hpp"
 #include "attention_host.hpp"
 
+#include <algorithm>
+
 using namespace aixd;
 using namespace aixk;
 using namespace aixk::attn;
@@ -22,8 +24,10 @@ struct BackwardArgs {
     float* delta;
     u32 tiles;                                // row tiles per head (dq), key tiles per key head (dk, dv)
     u32 splits;                               // shares of the queries (dk, dv)
+    u32 lead, lead_splits, lead_keys;         // key tiles with leading keys that a window does not hide: every query sees them, so they have more shares
     i32 whole_dq, whole_dk, whole_dv;
-    float* part;                              // [split][dk, dv][batch * key heads * keys][DP]
+    float* part;                              // [split][dk, dv][batch * key heads * keys][DP] if there are several; the lead tiles' further shares
+                                              // follow, [share][dk, dv][batch * key heads * lead_keys][DP] (see share_of)
 };
 
 // As in attention_k the scores are transposed (a lane = one query): dS^T, rounded, feeds dq^T = K^T dS^T as it lies.
@@ -108,6 +112,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
             f32x16 x = f32x16{}, dp = f32x16{};
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
+                if (past<T>(c * 16, s.DW)) break;
                 x = M::run32(L::row(ks, kb * 32 + (lane & 31), 2 * c + half), q[c], x);
                 dp = M::run32(L::row(vs, kb * 32 + (lane & 31), 2 * c + half), go[c], dp);
             }
@@ -125,7 +130,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
             for (int c = 0; c < 2; ++c) {
                 const Frag ds = M::pack8(e + 8 * c);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = M::run32(L::column(ks, kb * 32 + c * 16, d, lane), ds, acc[d]);
+                for (int d = 0; d < DB; ++d) if (!past<T>(d * 32, s.DW)) acc[d] = M::run32(L::column(ks, kb * 32 + c * 16, d, lane), ds, acc[d]);
             }
         }
     }
@@ -138,17 +143,37 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
             put4<T>(row, a.dq.d, a.whole_dq, d * 32 + g * 8 + half * 4, s.D, acc[d][4 * g] * s.scale, acc[d][4 * g + 1] * s.scale, acc[d][4 * g + 2] * s.scale, acc[d][4 * g + 3] * s.scale);
 }
 
-// A wave keeps 32 keys, its 32 values (in LDS where a row is 256 bytes or more: the registers then hold two waves per SIMD) and
-// both sums; the queries and gradients of every head of the group come by in tiles of QT rows.  Here a lane is one key: P and
+// A wave keeps both sums of its 32 keys in registers, and the keys and values where the registers hold them beside that.  Rows of
+// 256 bytes: sums of 128 registers leave room for two waves per SIMD only with keys and values in LDS (32 more registers for the
+// keys alone cost eight spilled ones and 18 %: each reload waits for the loads in flight), 144 KB for eight waves; one wave
+// per SIMD with everything in registers takes 1.4 times as long.  The queries and gradients of every head of the group come by in tiles of QT rows.  Here a lane is one key: P and
 // dS, rounded, feed dv^T = grad^T P and dk^T = q^T dS as they lie.
 template <class T, int DP> struct KeyBlock {
-    static constexpr bool kValuesInLds = DP * sizeof(T) >= 256 && DP * sizeof(T) <= 512;
-    static constexpr int kRows = DP * sizeof(T) <= 128 ? 64 : 32;                      // QT
-    static constexpr size_t kLds = 2 * (size_t)kRows * DP * sizeof(T) + 2 * kRows * sizeof(float) + (kValuesInLds ? 128 * DP * sizeof(T) : 0);
+    static constexpr size_t kRow = DP * sizeof(T);
+    static constexpr int kThreads = kRow == 256 ? 512 : 256, kKeys = kThreads / 2;
+    static constexpr int kWaves = kRow <= 256 ? 2 : 1;                                   // per SIMD
+    static constexpr bool kKeysInLds = kRow == 256, kValuesInLds = kRow >= 256 && kRow <= 512;
+    static constexpr int kRows = kRow <= 128 ? 64 : 32;                                  // QT
+    static constexpr size_t kLds = 2 * kRows * kRow + 2 * kRows * sizeof(float) + (kKeysInLds + kValuesInLds) * kKeys * kRow;
 };
-template <class T, int DP, int QT>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dkdv_k(BackwardArgs a)
+// where share `split` of key j of a (batch, key head) lies
+template <int DP> __device__ __forceinline__ void share_of(const BackwardArgs& a, u32 split, u64 head, u32 j, float** pk, float** pv)
 {
+    const u64 heads = (u64)a.s.B * a.s.HK, lead_rows = heads * a.lead_keys;
+    const u64 rows = a.splits > 1 ? heads * (u32)a.s.SK : 0;
+    if (a.splits > 1 && split < a.splits) {
+        *pk = a.part + ((u64)split * 2 * rows + head * (u32)a.s.SK + j) * DP;
+        *pv = *pk + rows * DP;
+    } else {
+        *pk = a.part + ((u64)a.splits * 2 * rows + (u64)(a.splits > 1 ? split - a.splits : split) * 2 * lead_rows + head * a.lead_keys + j) * DP;
+        *pv = *pk + lead_rows * DP;
+    }
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWaves)) void attention_dkdv_k(BackwardArgs a)
+{
+    constexpr int NT = KeyBlock<T, DP>::kThreads, KB = KeyBlock<T, DP>::kKeys, QT = KeyBlock<T, DP>::kRows;
     typedef Mma<T> M;
     typedef typename M::Frag Frag;
     typedef Tile<T, DP> L;
@@ -158,38 +183,51 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dkdv
     char* gs = lds + QT * L::PITCH;
     float* ls = (float*)(lds + 2 * QT * L::PITCH);            // lse (log2), delta of the tile's rows
     float* ds = ls + QT;
-    constexpr bool VL = KeyBlock<T, DP>::kValuesInLds;
-    char* vs = (char*)(ds + QT);                              // the values of all 128 keys, if they are kept here
+    constexpr bool KL = KeyBlock<T, DP>::kKeysInLds, VL = KeyBlock<T, DP>::kValuesInLds;
+    char* vs = (char*)(ds + QT);                              // the values and keys of the block, if they are kept here
+    char* ks = vs + KB * L::PITCH;
     const Shape& s = a.s;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    const u32 id = xcd_order(blockIdx.x, gridDim.x), split = id % a.splits, rest = id / a.splits;
-    const u32 head = rest / a.tiles, tile = rest % a.tiles;
+    // a head's workgroups: the lead tiles with lead_splits shares each, then the others with `splits`
+    const u32 per_head = a.lead * a.lead_splits + (a.tiles - a.lead) * a.splits;
+    const u32 id = xcd_order(blockIdx.x, gridDim.x), head = id / per_head, in = id % per_head;
+    const bool leads = in < a.lead * a.lead_splits;
+    const u32 splits = leads ? a.lead_splits : a.splits, in2 = leads ? in : in - a.lead * a.lead_splits;
+    const u32 split = in2 % splits, tile = in2 / splits + (leads ? 0 : a.lead);
     const u32 b = head / s.HK, hk = head % s.HK;
     const Row r = row_of(s, b);
-    const i32 k0 = (i32)tile * 128, k1 = k0 + 127 < r.length - 1 ? k0 + 127 : r.length - 1;      // keys in use
+    const i32 k0 = (i32)tile * KB, k1 = k0 + KB - 1 < r.length - 1 ? k0 + KB - 1 : r.length - 1;      // keys in use
     const i32 j0 = k0 + wave * 32, j = j0 + (lane & 31);
     const bool on = j < r.length;
 
-    Frag kf[DC], vf[VL ? 1 : DC];
+    Frag kf[KL ? 1 : DC], vf[VL ? 1 : DC];
     {
         const u64 row = (u64)(u32)(on ? j : 0);
         const T* rk = (const T*)a.k.p + b * a.k.b + hk * a.k.h + row * a.k.s;
         const T* rv = (const T*)a.v.p + b * a.v.b + hk * a.v.h + row * a.v.s;
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
-            kf[c] = load8<T>(rk, c * 16 + half * 8, s.DW, on);
+            if constexpr (!KL) kf[c] = load8<T>(rk, c * 16 + half * 8, s.DW, on);
             if constexpr (!VL) vf[c] = load8<T>(rv, c * 16 + half * 8, s.DW, on);
         }
     }
     if constexpr (VL) {                                       // (each wave reads its own rows only, but the loop's first barrier comes in between anyway)
         if (k0 <= k1) {
-            Stage<T, DP, 128, 256> sv;
+            Stage<T, DP, KB, NT> sv;
             sv.load((const T*)a.v.p + b * a.v.b + hk * a.v.h, a.v.s, k0, r.length, s.DW, tid);
             sv.store(vs, k0, r.length, s.DW, tid);
+            if constexpr (KL) {
+                sv.load((const T*)a.k.p + b * a.k.b + hk * a.k.h, a.k.s, k0, r.length, s.DW, tid);
+                sv.store(ks, k0, r.length, s.DW, tid);
+            }
         }
     }
+    auto key = [&](int c) {
+        if constexpr (KL) return L::row(ks, wave * 32 + (lane & 31), 2 * c + half);
+        else return kf[c];
+    };
     auto value = [&](int c) {
         if constexpr (VL) return L::row(vs, wave * 32 + (lane & 31), 2 * c + half);
         else return vf[c];
@@ -213,12 +251,12 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dkdv
     const Queries seen = queries_of(s, r.length, j);
     const i32 first = i_lo / QT, per = i_lo < i_hi ? (i_hi + QT - 1) / QT - first : 0;
     const u64 total = (u64)(u32)per * s.G;
-    const u64 from = total * split / a.splits, to = total * (split + 1) / a.splits;
+    const u64 from = total * split / splits, to = total * (split + 1) / splits;
 
     // the (head of the group, tile) of a step, stepped on by counting (a division per step costs more than its products)
     struct At { u32 g; i32 tile; };
     auto on_from = [&](At& at) { if (++at.tile == per) { at.tile = 0; ++at.g; } };
-    Stage<T, DP, QT, 256> sq, sg;
+    Stage<T, DP, QT, NT> sq, sg;
     float next_l = 0.0f, next_d = 0.0f;
     auto load = [&](const At& at) {
         const u32 h = hk * s.G + at.g;
@@ -250,7 +288,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dkdv
             f32x16 x = f32x16{}, dp = f32x16{};
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
-                x = M::run32(L::row(qs, qb * 32 + (lane & 31), 2 * c + half), kf[c], x);
+                if (past<T>(c * 16, s.DW)) break;
+                x = M::run32(L::row(qs, qb * 32 + (lane & 31), 2 * c + half), key(c), x);
                 dp = M::run32(L::row(gs, qb * 32 + (lane & 31), 2 * c + half), value(c), dp);
             }
             const bool masked = !all_visible(s, r.length, r.start + q0, r.start + q1, j0, j0 + 31);
@@ -277,6 +316,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dkdv
                 const Frag fp = M::pack8(e + 8 * c), fs = M::pack8(w + 8 * c);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
+                    if (past<T>(d * 32, s.DW)) break;
                     dv[d] = M::run32(L::column(gs, qb * 32 + c * 16, d, lane), fp, dv[d]);
                     dk[d] = M::run32(L::column(qs, qb * 32 + c * 16, d, lane), fs, dk[d]);
                 }
@@ -284,10 +324,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dkdv
         }
     }
     if (j >= s.SK) return;
-    if (a.splits > 1) {
-        const u64 rows = (u64)s.B * s.HK * (u32)s.SK, at = (u64)head * (u32)s.SK + (u32)j;
-        float* pk = a.part + ((u64)split * 2 * rows + at) * DP;
-        float* pv = pk + rows * DP;
+    if (splits > 1) {
+        float *pk, *pv;
+        share_of<DP>(a, split, head, (u32)j, &pk, &pv);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -316,16 +355,19 @@ __global__ __launch_bounds__(256) void attention_dkdv_join_k(BackwardArgs a)
 {
     constexpr int LANES = DP / 4;
     const Shape& s = a.s;
-    const u64 rows = (u64)s.B * s.HK * (u32)s.SK;
     const u64 row = (u64)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const u32 keys = a.splits > 1 ? (u32)s.SK : a.lead_keys;       // per head, those with shares
     const u32 c = threadIdx.x % LANES * 4;
-    if (row >= rows) return;
+    if (row >= (u64)s.B * s.HK * keys) return;
+    const u64 j = row % keys, head = row / keys, hk = head % s.HK, b = head / s.HK;
     f32x4 k = f32x4{}, v = f32x4{};
-    for (u32 n = 0; n < a.splits; ++n) {
-        k += *(const f32x4*)(a.part + (((u64)n * 2) * rows + row) * DP + c);
-        v += *(const f32x4*)(a.part + (((u64)n * 2 + 1) * rows + row) * DP + c);
+    const u32 splits = j < a.lead_keys ? a.lead_splits : a.splits;
+    for (u32 n = 0; n < splits; ++n) {
+        float *pk, *pv;
+        share_of<DP>(a, n, head, (u32)j, &pk, &pv);
+        k += *(const f32x4*)(pk + c);
+        v += *(const f32x4*)(pv + c);
     }
-    const u64 j = row % (u32)s.SK, head = row / (u32)s.SK, hk = head % s.HK, b = head / s.HK;
     put4<T>(a.dk.p + (b * a.dk.b + hk * a.dk.h + j * a.dk.s) * sizeof(T), a.dk.d, a.whole_dk, c, s.D, k.x * s.scale, k.y * s.scale, k.z * s.scale, k.w * s.scale);
     put4<T>(a.dv.p + (b * a.dv.b + hk * a.dv.h + j * a.dv.s) * sizeof(T), a.dv.d, a.whole_dv, c, s.D, v.x, v.y, v.z, v.w);
 }
@@ -345,28 +387,46 @@ template <class T, int DP> int backward(aixk_ctx* ctx, const Call& c, BackwardAr
         AIXK_HIP(hipGetLastError());
     }
     if (s.SK == 0 || s.B == 0 || s.HK == 0) return AIXK_OK;
-    a.tiles = ((u32)s.SK + 127) / 128;
-    const u64 grid = (u64)s.B * s.HK * a.tiles, rows = (u64)s.B * s.HK * (u32)s.SK;
-    // Shares of the queries until there are two workgroups per compute unit, each of at least 512 queries.
-    u64 splits = ((u64)ctx->cus * 2 + grid - 1) / grid;
-    const u64 most = ((u64)s.G * (u32)s.SQ + 511) / 512;
-    if (splits > most) splits = most;
-    if (splits < 1) splits = 1;
-    AIXK_REQUIRE(grid * splits < (1ull << 31), "attention_backward: too many rows");
+    constexpr u32 keys = KeyBlock<T, DP>::kKeys;
+    a.tiles = ((u32)s.SK + keys - 1) / keys;
+    const u64 heads = (u64)s.B * s.HK, rows = heads * (u32)s.SK;
+    // Shares of the queries by a cost in microseconds: rounds of workgroups, each of its steps (about 2 us, three of them the
+    // workgroup's own), and the shares written and read again (4 TB/s, and the joining launch).  Key tiles with leading keys, which
+    // every query sees, take as many more shares as they have more queries.  16 heads on 4 of 4096 x 128, window 1024: 3 shares
+    // SHARE3_US, 8 shares 148 us.
+    constexpr u64 resident = KeyBlock<T, DP>::kWaves * 256 / KeyBlock<T, DP>::kThreads;
+    const u64 slots = (u64)ctx->cus * resident;
+    const u64 seen = s.window && (u64)s.window + keys < (u64)(u32)s.SQ ? (u64)s.window + keys : (u64)(u32)s.SQ;      // queries of a tile at most
+    const u64 steps = ((u64)s.G * seen + KeyBlock<T, DP>::kRows - 1) / KeyBlock<T, DP>::kRows, more = seen ? std::min<u64>(((u32)s.SQ + seen - 1) / seen, 32) : 1;
+    if (s.window && s.sinks && seen) {
+        a.lead = ((u32)s.sinks + keys - 1) / keys;
+        if (a.lead > a.tiles) a.lead = a.tiles;
+        a.lead_keys = a.lead * keys < (u32)s.SK ? a.lead * keys : (u32)s.SK;
+    }
+    u64 splits = 1, planes = 0, grid = 0;
+    double least = 0.0;
+    for (u64 sp = 1; sp <= 64 && (sp == 1 || sp * 4 <= steps); ++sp) {
+        const u64 n = heads * (a.lead * sp * more + (a.tiles - a.lead) * sp);
+        const u64 shares = (sp > 1 ? sp * rows : 0) + (sp * more > 1 ? (sp > 1 ? sp * (more - 1) : more) * heads * a.lead_keys : 0);
+        const double cost = 2.0 * (double)((n + slots - 1) / slots) * (double)((steps + sp - 1) / sp + 3) + (shares ? 3.0 + (double)shares * (16.0 * DP / 4e6) : 0.0);
+        if (sp == 1 || cost < least) { least = cost; splits = sp; planes = shares; grid = n; }
+    }
     a.splits = (u32)splits;
-    if (splits > 1) {
+    a.lead_splits = (u32)(a.lead ? splits * more : splits);
+    AIXK_REQUIRE(grid < (1ull << 31), "attention_backward: too many rows");
+    if (planes) {
         void* ws;
-        AIXK_TRY(block_scratch(ctx, kScratchParts, (size_t)splits * 2 * rows * DP * sizeof(float), &ws));
+        AIXK_TRY(block_scratch(ctx, kScratchParts, (size_t)planes * 2 * DP * sizeof(float), &ws));
         a.part = (float*)ws;
     }
-    constexpr int QT = KeyBlock<T, DP>::kRows;
     constexpr size_t lds = KeyBlock<T, DP>::kLds;
-    AIXK_TRY(allow_lds(attention_dkdv_k<T, DP, QT>, lds));
-    hipLaunchKernelGGL((attention_dkdv_k<T, DP, QT>), dim3((unsigned)(grid * splits)), dim3(256), lds, ctx->stream, a);
+    AIXK_TRY(allow_lds(attention_dkdv_k<T, DP>, lds));
+    hipLaunchKernelGGL((attention_dkdv_k<T, DP>), dim3((unsigned)grid), dim3(KeyBlock<T, DP>::kThreads), lds, ctx->stream, a);
     AIXK_HIP(hipGetLastError());
-    if (splits > 1) {
+    if (a.part) {
         constexpr u32 per = 256 / (DP / 4);
-        hipLaunchKernelGGL((attention_dkdv_join_k<T, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, ctx->stream, a);
+        const u64 joined = heads * (splits > 1 ? (u64)(u32)s.SK : a.lead_keys);
+        hipLaunchKernelGGL((attention_dkdv_join_k<T, DP>), dim3((unsigned)((joined + per - 1) / per)), dim3(256), 0, ctx->stream, a);
         AIXK_HIP(hipGetLastError());
     }
     return AIXK_OK;
@@ -405,6 +465,6 @@ extern "C" int32_t aixk_attention_backward(aixk_ctx* ctx, const aixhip_tensor* g
     AIXK_TRY(c.operand(ctx, out, kScratchOut, &c.y));
     void* delta;
     AIXK_TRY(block_scratch(ctx, kScratchDelta, (size_t)(numel(lse) + 1) * sizeof(float), &delta));
-    BackwardArgs a{c.s, c.grad, c.q, c.k, c.v, c.y, c.dq, c.dk, c.dv, c.lse, (float*)delta, 0, 1, wq, wk, wv, nullptr};
+    BackwardArgs a{c.s, c.grad, c.q, c.k, c.v, c.y, c.dq, c.dk, c.dv, c.lse, (float*)delta, 0, 1, 0, 1, 0, wq, wk, wv, nullptr};
     return c.by_type([&](auto type, auto width) { return backward<decltype(type), decltype(width)::value>(ctx, c, a); });
 }
