@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
         for (int kb = 0; kb < 2; ++kb) {
             x[kb] = f32x16{};
 #pragma unroll
-            for (int c = 0; c < DC; ++c) x[kb] = M::run32(L::row(ks, kb * 32 + (lane & 31), 2 * c + half), q[c], x[kb]);
+            for (int c = 0; c < DC; ++c) if (!past<T, DP>(c * 16, s.DW)) x[kb] = M::run32(L::row(ks, kb * 32 + (lane & 31), 2 * c + half), q[c], x[kb]);
         }
         if (!all_visible(s, r.length, r.start + w0, r.start + w1, j0, j0 + KT - 1)) {
 #pragma unroll
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] = M::run32(L::column(vs, c * 16, d, lane), w[c], o[d]);
+            for (int d = 0; d < DB; ++d) if (!past<T, DP>(d * 32, s.DW)) o[d] = M::run32(L::column(vs, c * 16, d, lane), w[c], o[d]);
     }
 
     l += other_half(l);
@@ -154,12 +154,12 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
 // fast (a wave of 32 queries takes 7 us for a tile of 64 keys: half the queries are twice the waves to fill the chip with, and
 // the head dim's tail is left out), and for grids of 128-query workgroups that leave compute units without one.
 template <class T, int DP>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention16_k(ForwardArgs a)
+__global__ __launch_bounds__(256, DP * sizeof(T) <= 512 ? 2 : 1) void attention16_k(ForwardArgs a)
 {
     typedef Mma<T> M;
     typedef typename M::Frag Frag;
     typedef Tile<T, DP> L;
-    constexpr int KT = DP * sizeof(T) <= 512 ? 64 : 32, SUB = KT / 16, DB = DP / 16, DC = DP / 32;
+    constexpr int KT = DP * sizeof(T) <= 256 ? 64 : 32, SUB = KT / 16, DB = DP / 16, DC = DP / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     char* ks = lds;
     char* vs = lds + KT * L::PITCH;
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention16_k(
         for (int k = 0; k < SUB; ++k) x[k] = f32x4{};
 #pragma unroll
         for (int c = 0; c < DC; ++c) {
-            if (past<T>(c * 32, s.DW)) break;
+            if (past<T, DP>(c * 32, s.DW)) break;
 #pragma unroll
             for (int k = 0; k < SUB; ++k) x[k] = M::run16(L::row(ks, k * 16 + c15, 4 * c + g), q[c], x[k]);
         }
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention16_k(
             const Frag w = M::pack8(e);
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                if (past<T>(d * 16, s.DW)) break;
+                if (past<T, DP>(d * 16, s.DW)) break;
                 o[d] = M::run16(L::column16(vs, k * 32, d, lane), w, o[d]);
             }
         }
@@ -277,20 +277,22 @@ struct SplitArgs {
     float* part_ml;                           // [split][batch * heads * queries][2]: maximum (log2), sum
 };
 
-constexpr int kSplitWaves = 4, kSplitKeys = 32;        // keys per wave and step
+constexpr int kSplitKeys = 32;        // keys per wave and step
 
-template <class T, int DP> struct SplitLds {
+// WAVES: 4, several workgroups to a row's keys; or as many as the registers allow for one workgroup that takes all of them
+template <class T, int DP, int WAVES> struct SplitLds {
     static constexpr int kSlab = kSplitKeys * DP * (int)sizeof(T);                        // a wave's keys of V
-    static constexpr int kJoin = kSplitWaves * (16 * DP + 32) * 4;                           // accumulators, maxima and sums of all waves
-    static constexpr int kBytes = kSlab * kSplitWaves > kJoin ? kSlab * kSplitWaves : kJoin;
+    static constexpr int kJoin = WAVES * (16 * DP + 32) * 4;                                 // accumulators, maxima and sums of all waves
+    static constexpr int kBytes = kSlab * WAVES > kJoin ? kSlab * WAVES : kJoin;
 };
+template <class T, int DP> constexpr int most_waves() { return DP * sizeof(T) <= 128 ? 16 : DP * sizeof(T) <= 256 ? 8 : 4; }
 
 // Row r of a key head's R = G * SQ rows is query r % SQ of head r / SQ of the group.  16 rows against 32 keys with v_mfma
 // 16x16: keys are read from memory straight as the first operand; V goes through a slab of LDS that belongs to the wave
 // alone (no barrier in the loop) to be read transposed.  Reading the cache is the bound, so the next step's words are in
 // flight while a step is computed.
-template <class T, int DP>
-__global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs a)
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attention_split_k(SplitArgs a)
 {
     typedef Mma<T> M;
     typedef typename M::Frag Frag;
@@ -300,7 +302,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs 
     const Shape& s = a.s;
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c15 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    char* slab = lds + wave * SplitLds<T, DP>::kSlab;
+    char* slab = lds + wave * SplitLds<T, DP, WAVES>::kSlab;
 
     const u32 id = blockIdx.x, split = id % a.splits, rest = id / a.splits;
     const u32 tile = rest % a.tiles, bk = rest / a.tiles, b = bk / s.HK, hk = bk % s.HK;
@@ -361,7 +363,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs 
     };
     i32 n = from + wave;
     if (n < to) load(tile_at(t, n) * KT);
-    for (; n < to; n += kSplitWaves) {
+    for (; n < to; n += WAVES) {
         const i32 j0 = tile_at(t, n) * KT;
         f32x4 x[2];
 #pragma unroll
@@ -369,6 +371,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs 
             x[kb] = f32x4{};
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
+                if (past<T, DP>(c * 32, s.DW)) break;
                 // (words past the head dim repeat the last one: the query's zeros would meet an infinity there as a NaN)
                 Frag f = kf[kb][c];
                 if constexpr (sizeof(T) == 2) { if (c * 32 + g * 8 >= (int)s.DW) f = M::zero(); }
@@ -381,7 +384,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs 
             const int at = lane + e * 64, k = at / WORDS, w = at % WORDS;
             *(u32x4*)(slab + k * PITCH + ((w ^ turn(k)) << 4)) = j0 + k < r.length && w <= last ? vf[e] : u32x4{0, 0, 0, 0};
         }
-        if (n + kSplitWaves < to) load(tile_at(t, n + kSplitWaves) * KT);
+        if (n + WAVES < to) load(tile_at(t, n + WAVES) * KT);
 
         float top = -__builtin_inff();
 #pragma unroll
@@ -413,6 +416,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs 
         // column 16 d + lane % 16 of V, the keys 16 (j / 4) + 4 g + j % 4 of element j
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
+            if (past<T, DP>(d * 16, s.DW)) break;
             Frag f;
             if constexpr (sizeof(T) == 2) {
                 const int k = 4 * g + (c15 >> 2), word = 2 * d + ((c15 & 3) >> 1);
@@ -437,23 +441,23 @@ __global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs 
     // the waves' shares: [wave][16 rows][DP] accumulators, then maxima and sums
     __syncthreads();
     float* all = (float*)lds;
-    float* ml = all + kSplitWaves * 16 * DP;
+    float* ml = all + WAVES * 16 * DP;
 #pragma unroll
     for (int d = 0; d < DB; ++d) *(f32x4*)(all + (wave * 16 + c15) * DP + ((d * 16 + 4 * g) ^ (4 * (c15 & 7)))) = o[d];
     if (g == 0) { ml[(wave * 16 + c15) * 2] = m; ml[(wave * 16 + c15) * 2 + 1] = l; }
     __syncthreads();
     const u64 rows = (u64)s.B * s.H * (u32)s.SQ;
-    for (int e = tid; e < 16 * DP / 4; e += kSplitWaves * 64) {
+    for (int e = tid; e < 16 * DP / 4; e += WAVES * 64) {
         const int row = e / (DP / 4), d = e % (DP / 4) * 4;
         if (r0 + row >= R) continue;
         float top = -__builtin_inff();
 #pragma unroll
-        for (int w = 0; w < kSplitWaves; ++w) top = fmaxf(top, ml[(w * 16 + row) * 2]);
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ml[(w * 16 + row) * 2]);
         f32x4 sum = f32x4{};
         float total = 0.0f;
         if (top != -__builtin_inff()) {
 #pragma unroll
-            for (int w = 0; w < kSplitWaves; ++w) {
+            for (int w = 0; w < WAVES; ++w) {
                 const float f = exp2_of(ml[(w * 16 + row) * 2] - top);
                 total += f * ml[(w * 16 + row) * 2 + 1];
                 sum += f * *(const f32x4*)(all + (w * 16 + row) * DP + (d ^ (4 * (row & 7))));
@@ -472,28 +476,36 @@ __global__ __launch_bounds__(kSplitWaves * 64) void attention_split_k(SplitArgs 
     }
 }
 
-// the shares of the keys added up in their order: 64 lanes on DP / 4 groups of four, four rows per workgroup
+// The shares of the keys added up: a workgroup per row, DP / 4 lanes side by side in several groups that take the shares in turn
+// and meet in LDS (one group alone waits for a load per share: 9.2 us for 512 rows of 8 shares).
 template <class T, int DP>
 __global__ __launch_bounds__(256) void attention_join_k(SplitArgs a)
 {
-    constexpr int LANES = DP / 4;                              // lanes per row
+    constexpr int LANES = DP / 4, GROUPS = 256 / LANES;
+    __shared__ f32x4 part[GROUPS][LANES];
     const Shape& s = a.s;
-    const u64 rows = (u64)s.B * s.H * (u32)s.SQ;
-    const u64 at = (u64)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const u32 d = threadIdx.x % LANES * 4;
-    if (at >= rows) return;
-    float top = -__builtin_inff();
+    const u64 rows = (u64)s.B * s.H * (u32)s.SQ, at = blockIdx.x;
+    const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const u32 d = lane * 4;
+    float top = -__builtin_inff(), total = 0.0f;
+#pragma unroll 8
     for (u32 k = 0; k < a.splits; ++k) top = fmaxf(top, a.part_ml[(k * rows + at) * 2]);
     f32x4 sum = f32x4{};
-    float total = 0.0f;
     if (top != -__builtin_inff()) {
+#pragma unroll 8
         for (u32 k = 0; k < a.splits; ++k) {
             const f32x2 ml = *(const f32x2*)(a.part_ml + (k * rows + at) * 2);
-            const float f = exp2_of(ml.x - top);
-            total += f * ml.y;
-            sum += f * *(const f32x4*)(a.part_o + (k * rows + at) * DP + d);
+            total += exp2_of(ml.x - top) * ml.y;
         }
+#pragma unroll 2
+        for (u32 k = group; k < a.splits; k += GROUPS)
+            sum += exp2_of(a.part_ml[(k * rows + at) * 2] - top) * *(const f32x4*)(a.part_o + (k * rows + at) * DP + d);
     }
+    part[group][lane] = sum;
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) sum += part[g][lane];
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (a.lse && d == 0) a.lse[at] = total == 0.0f ? -__builtin_inff() : (top + log2f(total)) * kLn2;
     const u32 i = (u32)(at % (u32)s.SQ), h = (u32)(at / (u32)s.SQ % s.H), b = (u32)(at / (u32)s.SQ / s.H);
@@ -543,7 +555,7 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
             const u64 grid = (u64)s.B * s.H * (((u32)s.SQ + 63) / 64);
             AIXK_REQUIRE(grid < (1ull << 31), "attention: too many rows");
             ForwardArgs a{s, c.q, c.k, c.v, c.out, c.lse, ((u32)s.SQ + 63) / 64, c.whole_out};
-            constexpr size_t lds = 2 * (DP * sizeof(T) <= 512 ? 64 : 32) * DP * sizeof(T);
+            constexpr size_t lds = 2 * (DP * sizeof(T) <= 256 ? 64 : 32) * DP * sizeof(T);
             AIXK_TRY(allow_lds(attention16_k<T, DP>, lds));
             hipLaunchKernelGGL((attention16_k<T, DP>), dim3((unsigned)grid), dim3(256), lds, ctx->stream, a);
             AIXK_HIP(hipGetLastError());
@@ -560,11 +572,24 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
         }
     }
     SplitArgs a{s, c.q, c.k, c.v, c.out, c.lse, (R + 15) / 16, 1, c.whole_out, nullptr, nullptr};
-    // Shares of the keys until every compute unit has four workgroups, but no share below one step of all waves.  What a row
-    // can see at most bounds the steps: the whole cache, or the window and the leading keys.
+    auto launch = [&](auto waves_tag) -> int {
+        constexpr int WAVES = decltype(waves_tag)::value;
+        constexpr size_t lds = SplitLds<T, DP, WAVES>::kBytes;
+        AIXK_TRY(allow_lds(attention_split_k<T, DP, WAVES>, lds));
+        hipLaunchKernelGGL((attention_split_k<T, DP, WAVES>), dim3((unsigned)(narrow * a.splits)), dim3(WAVES * 64), lds, ctx->stream, a);
+        AIXK_HIP(hipGetLastError());
+        return AIXK_OK;
+    };
+    AIXK_REQUIRE(narrow < (1ull << 31) && rows < (1ull << 31), "attention: too many rows");
+    // What a row can see at most bounds its steps: the whole cache, or the window and the leading keys.
     u64 keys = (u64)s.SK;
     if (s.window && (u64)s.window + (u64)s.SQ + (u64)s.sinks < keys) keys = (u64)s.window + (u64)s.SQ + (u64)s.sinks;
-    const u64 steps = (keys + kSplitKeys * kSplitWaves - 1) / (kSplitKeys * kSplitWaves);
+    // Few keys and few workgroups: one workgroup of as many waves as it holds takes them all in at most three steps, where
+    // sharing them out costs a second launch (12 heads of 64 on 512 keys: ONE_US us, in 4 shares 8.3).
+    constexpr int most = most_waves<T, DP>();
+    if (most > 4 && narrow < (u64)ctx->cus && keys > 4 * kSplitKeys && keys <= 3u * most * kSplitKeys) return launch(std::integral_constant<int, most>{});
+    // Otherwise shares of the keys until every compute unit has four workgroups, but no share below one step of all waves.
+    const u64 steps = (keys + kSplitKeys * 4 - 1) / (kSplitKeys * 4);
     u64 splits = ((u64)ctx->cus * 4 + narrow - 1) / narrow;
     if (splits > steps) splits = steps;
     if (splits < 1) splits = 1;
@@ -577,13 +602,9 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
         a.part_o = (float*)ws;
         a.part_ml = (float*)((char*)ws + o_bytes);
     }
-    constexpr size_t lds = SplitLds<T, DP>::kBytes;
-    AIXK_TRY(allow_lds(attention_split_k<T, DP>, lds));
-    hipLaunchKernelGGL((attention_split_k<T, DP>), dim3((unsigned)(narrow * splits)), dim3(kSplitWaves * 64), lds, ctx->stream, a);
-    AIXK_HIP(hipGetLastError());
+    AIXK_TRY(launch(std::integral_constant<int, 4>{}));
     if (splits > 1) {
-        constexpr u32 per = 256 / (DP / 4);
-        hipLaunchKernelGGL((attention_join_k<T, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, ctx->stream, a);
+        hipLaunchKernelGGL((attention_join_k<T, DP>), dim3((unsigned)rows), dim3(256), 0, ctx->stream, a);
         AIXK_HIP(hipGetLastError());
     }
     return AIXK_OK;

@@ -193,8 +193,9 @@ template <class T> __device__ __forceinline__ typename Mma<T>::Frag load8(const 
 }
 
 // Elements from d on lie past the head dim and their products are left out: f32, whose matrix instructions take 16 times as
-// long as the branch's; the 16-bit kernels multiply the zeros, which keeps their loops free of branches.
-template <class T> __device__ __forceinline__ bool past(int d, u32 DW) { return sizeof(T) == 4 && d >= (int)DW; }
+// long as the branch does, and head dims above 128, where the branches also keep the compiler from holding every operand of a
+// loop at once (attention_dkdv_k at 256: SPILLS).  The other kernels multiply the zeros and stay free of branches.
+template <class T, int DP> __device__ __forceinline__ bool past(int d, u32 DW) { return (sizeof(T) == 4 || DP > 128) && d >= (int)DW; }
 
 // Waves per SIMD a kernel is compiled for: two where a wave's share of the 512 registers then holds its accumulators, fragments
 // and staged words (rows of up to 256 bytes), else one.  Two waves cover each other's exponentials, barriers and LDS reads:

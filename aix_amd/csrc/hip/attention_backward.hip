@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
             f32x16 x = f32x16{}, dp = f32x16{};
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
-                if (past<T>(c * 16, s.DW)) break;
+                if (past<T, DP>(c * 16, s.DW)) break;
                 x = M::run32(L::row(ks, kb * 32 + (lane & 31), 2 * c + half), q[c], x);
                 dp = M::run32(L::row(vs, kb * 32 + (lane & 31), 2 * c + half), go[c], dp);
             }
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
             for (int c = 0; c < 2; ++c) {
                 const Frag ds = M::pack8(e + 8 * c);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) if (!past<T>(d * 32, s.DW)) acc[d] = M::run32(L::column(ks, kb * 32 + c * 16, d, lane), ds, acc[d]);
+                for (int d = 0; d < DB; ++d) if (!past<T, DP>(d * 32, s.DW)) acc[d] = M::run32(L::column(ks, kb * 32 + c * 16, d, lane), ds, acc[d]);
             }
         }
     }
@@ -288,7 +288,7 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
             f32x16 x = f32x16{}, dp = f32x16{};
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
-                if (past<T>(c * 16, s.DW)) break;
+                if (past<T, DP>(c * 16, s.DW)) break;
                 x = M::run32(L::row(qs, qb * 32 + (lane & 31), 2 * c + half), key(c), x);
                 dp = M::run32(L::row(gs, qb * 32 + (lane & 31), 2 * c + half), value(c), dp);
             }
@@ -316,7 +316,7 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
                 const Frag fp = M::pack8(e + 8 * c), fs = M::pack8(w + 8 * c);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    if (past<T>(d * 32, s.DW)) break;
+                    if (past<T, DP>(d * 32, s.DW)) break;
                     dv[d] = M::run32(L::column(gs, qb * 32 + c * 16, d, lane), fp, dv[d]);
                     dk[d] = M::run32(L::column(qs, qb * 32 + c * 16, d, lane), fs, dk[d]);
                 }

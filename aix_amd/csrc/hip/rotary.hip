@@ -212,20 +212,22 @@ extern "C" int32_t aixk_rotary(aixk_ctx* ctx, const aixhip_tensor* q, const aixh
     a.positions = (const i32*)positions->data + positions->offset; a.pb = positions->strides[0]; a.ps = positions->strides[1];
     a.S = S; a.rows = B * S; a.HQ = (u32)HQ; a.HK = (u32)HK; a.D = (u32)D; a.pairs = (u32)pairs;
     a.inverse = spec->inverse != 0; a.magnitude = spec->magnitude;
-    const double two_pi = 6.283185307179586476925286766559;
+    // the frequencies are a geometric series, stepped in extended precision (a power per pair takes the host longer than the
+    // kernel takes for a token)
     double base = spec->base;
     if (spec->scaling == AIXK_ROTARY_BASE && spec->dims > 2) base *= std::pow(spec->factor, (double)spec->dims / ((double)spec->dims - 2.0));
-    for (uint64_t i = 0; i < pairs; ++i) {
-        double f = std::pow(base, -2.0 * (double)i / (double)spec->dims);
-        if (spec->scaling == AIXK_ROTARY_LINEAR) f /= spec->factor;
+    const long double ratio = powl((long double)base, -2.0L / (long double)spec->dims), per_turn = 0.15915494309189533576888L;      // 1 / (2 pi)
+    long double f = 1.0L;
+    for (uint64_t i = 0; i < pairs; ++i, f *= ratio) {
+        long double turns = f * per_turn;
+        if (spec->scaling == AIXK_ROTARY_LINEAR) turns /= (long double)spec->factor;
         if (spec->scaling == AIXK_ROTARY_PARTS) {
-            double kept = (spec->original_length * f / two_pi - spec->low_turns) / (spec->high_turns - spec->low_turns);
+            double kept = (spec->original_length * (double)turns - spec->low_turns) / (spec->high_turns - spec->low_turns);
             kept = kept < 0.0 ? 0.0 : kept > 1.0 ? 1.0 : kept;
-            f = f * (kept + (1.0 - kept) / spec->factor);
+            turns *= (long double)(kept + (1.0 - kept) / spec->factor);
         }
-        const long double turns = (long double)f / 6.283185307179586476925286766559005768L;
-        const long double part = turns - floorl(turns);                        // whole turns per position do nothing
-        a.turn[i] = (u64)(part * 18446744073709551616.0L);
+        if (turns >= 1.0L) turns -= floorl(turns);                             // whole turns per position do nothing
+        a.turn[i] = (u64)(turns * 18446744073709551616.0L);
     }
     // Positions per workgroup: about 16 KB of elements, a table of at most 32 KB, and, if there are few positions, the heads
     // spread over workgroups until every compute unit has two.
