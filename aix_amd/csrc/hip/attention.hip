@@ -279,13 +279,13 @@ struct SplitArgs {
 
 constexpr int kSplitKeys = 32;        // keys per wave and step
 
-// WAVES: 4, several workgroups to a row's keys; or as many as the registers allow for one workgroup that takes all of them
+// WAVES: 4, several workgroups to a row's keys; or 8 for one workgroup that takes all of them
 template <class T, int DP, int WAVES> struct SplitLds {
     static constexpr int kSlab = kSplitKeys * DP * (int)sizeof(T);                        // a wave's keys of V
     static constexpr int kJoin = WAVES * (16 * DP + 32) * 4;                                 // accumulators, maxima and sums of all waves
     static constexpr int kBytes = kSlab * WAVES > kJoin ? kSlab * WAVES : kJoin;
 };
-template <class T, int DP> constexpr int most_waves() { return DP * sizeof(T) <= 128 ? 16 : DP * sizeof(T) <= 256 ? 8 : 4; }
+template <class T, int DP> constexpr int most_waves() { return DP * sizeof(T) <= 256 ? 8 : 4; }
 
 // Row r of a key head's R = G * SQ rows is query r % SQ of head r / SQ of the group.  16 rows against 32 keys with v_mfma
 // 16x16: keys are read from memory straight as the first operand; V goes through a slab of LDS that belongs to the wave
@@ -332,7 +332,8 @@ __global__ __launch_bounds__(WAVES * 64) void attention_split_k(SplitArgs a)
     // this workgroup's share of the visible steps; its waves take them in turn
     const Keys seen = keys_of(s, r.length, p);
     const Tiles t = tiles_of(s, r.length, p0, p1, KT);
-    const i32 from = (i32)((u64)(u32)t.n * split / a.splits), to = (i32)((u64)(u32)t.n * (split + 1) / a.splits);
+    const u32 each = (u32)t.n / a.splits, over = (u32)t.n % a.splits;
+    const i32 from = (i32)(split * each + (split < over ? split : over)), to = from + (i32)(each + (split < over ? 1 : 0));
 
     // slot of 16-byte word c of key k in the slab: the transposed reads take 32 bytes from each of eight keys at a time
     auto turn = [](int k) { return WORDS >= 16 ? ((k & 7) << 1) | ((k >> 3) & 1) : ((k >> 1) & 3) << 1; };
@@ -585,7 +586,7 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
     u64 keys = (u64)s.SK;
     if (s.window && (u64)s.window + (u64)s.SQ + (u64)s.sinks < keys) keys = (u64)s.window + (u64)s.SQ + (u64)s.sinks;
     // Few keys and few workgroups: one workgroup of as many waves as it holds takes them all in at most three steps, where
-    // sharing them out costs a second launch (12 heads of 64 on 512 keys: ONE_US us, in 4 shares 8.3).
+    // sharing them out costs a second launch (12 heads of 64 on 512 keys: 6.4 us with eight waves, 7.2 with sixteen, 4.8 + 3.4 in 4 shares).
     constexpr int most = most_waves<T, DP>();
     if (most > 4 && narrow < (u64)ctx->cus && keys > 4 * kSplitKeys && keys <= 3u * most * kSplitKeys) return launch(std::integral_constant<int, most>{});
     // Otherwise shares of the keys until every compute unit has four workgroups, but no share below one step of all waves.

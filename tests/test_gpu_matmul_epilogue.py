@@ -87,6 +87,14 @@ def test_whole_tiles(gpu, dtype, m, k, n, b_order):
     forward(gpu, dtype, m, k, n, b_order=b_order)
 
 
+@pytest.mark.parametrize("dtype", [O.BF16, O.F16])
+@pytest.mark.parametrize("m", [1, 7, 16, 17, 32, 33, 48, 64, 65])
+@pytest.mark.parametrize("k,n", [(8, 8), (40, 56), (256, 33), (776, 2048), (4104, 64), (8192, 16), (520, 8200)])
+@pytest.mark.parametrize("b_order", [(0, 1), (1, 0)])
+def test_few_rows(gpu, dtype, m, k, n, b_order):
+    forward(gpu, dtype, m, k, n, "silu", b_order=b_order)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("m,k,n", [(40, 72, 48), (9, 5, 11), (5, 8192, 64)])
