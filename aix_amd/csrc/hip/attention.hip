@@ -10,6 +10,8 @@
 #include "attention.hpp"
 #include "attention_host.hpp"
 
+#include <algorithm>
+
 using namespace aixd;
 using namespace aixk;
 using namespace aixk::attn;
@@ -111,7 +113,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int v = 0; v < 16; ++v) top = fmaxf(top, x[kb][v]);
-        top = fmaxf(top, other_half(top)) * c2;
+        top = max_of_halves(top) * c2;
         if (__any(top > m + 8.0f)) {                          // (m = -inf: any visible key)
             const float raised = fmaxf(m, top);
             const float keep = raised == -__builtin_inff() ? 0.0f : exp2_of(m - raised);
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
             for (int d = 0; d < DB; ++d) if (!past<T, DP>(d * 32, s.DW)) o[d] = M::run32(L::column(vs, c * 16, d, lane), w[c], o[d]);
     }
 
-    l += other_half(l);
+    l = sum_of_halves(l);
     if (!on) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;            // a row that sees nothing: zeros
     if (a.lse && half == 0) a.lse[((u64)b * s.H + h) * (u64)s.SQ + (u32)i] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * kLn2;
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 512 ? 2 : 1) void attention1
                 top = fmaxf(top, x[k][v]);
             }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64)) * c2;
+        top = max_of_halves(top) * c2;
         if (__any(top > m + 8.0f)) {
             const float raised = fmaxf(m, top);
             const float keep = raised == -__builtin_inff() ? 0.0f : exp2_of(m - raised);
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 512 ? 2 : 1) void attention1
         }
     }
     l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = sum_of_halves(l);
     if (!on) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (a.lse && g == 0) a.lse[((u64)b * s.H + h) * (u64)s.SQ + (u32)i] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * kLn2;
@@ -396,7 +398,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_split_k(SplitArgs a)
                 top = fmaxf(top, x[kb][v]);
             }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = max_of_halves(top);
         if (__any(top > m + 8.0f)) {
             const float raised = fmaxf(m, top);
             const float keep = raised == -__builtin_inff() ? 0.0f : exp2_of(m - raised);
@@ -437,7 +439,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_split_k(SplitArgs a)
         }
     }
     l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = sum_of_halves(l);
 
     // the waves' shares: [wave][16 rows][DP] accumulators, then maxima and sums
     __syncthreads();
@@ -589,9 +591,12 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
     // sharing them out costs a second launch (12 heads of 64 on 512 keys: 6.4 us with eight waves, 7.2 with sixteen, 4.8 + 3.4 in 4 shares).
     constexpr int most = most_waves<T, DP>();
     if (most > 4 && narrow < (u64)ctx->cus && keys > 4 * kSplitKeys && keys <= 3u * most * kSplitKeys) return launch(std::integral_constant<int, most>{});
-    // Otherwise shares of the keys until every compute unit has four workgroups, but no share below one step of all waves.
+    // Otherwise shares of the keys until every compute unit has four workgroups, but no share below one step of all waves; up to
+    // eight workgroups where a share still has eight steps (16 sequences of any length up to 32768: 193 us with shares for four
+    // workgroups, 172 for eight, which even the lengths out; 2052 keys: 31.0 us with four, 34.2 with eight).
     const u64 steps = (keys + kSplitKeys * 4 - 1) / (kSplitKeys * 4);
     u64 splits = ((u64)ctx->cus * 4 + narrow - 1) / narrow;
+    splits = std::max<u64>(splits, std::min<u64>(((u64)ctx->cus * 8 + narrow - 1) / narrow, steps / 8));
     if (splits > steps) splits = steps;
     if (splits < 1) splits = 1;
     AIXK_REQUIRE(narrow * splits < (1ull << 31), "attention: too many rows");

@@ -261,36 +261,58 @@ template <class T, int DP> struct Tile {
     }
 };
 
-// ROWS rows of DP elements on their way from memory into such a tile through the registers of NT threads: loads without
-// branches (the addresses stay inside the operand), zeros chosen when the words are stored.
+// ROWS rows of DP elements on their way from memory into such a tile through the registers of NT threads.  A tile whose rows
+// all exist and whose rows are DP elements is fetched from a uniform address and one offset per thread; at an edge the
+// addresses stay inside the operand and zeros are chosen when the words are stored.
 template <class T, int DP, int ROWS, int NT> struct Stage {
     typedef Tile<T, DP> L;
-    static constexpr int N = ROWS * L::WORDS / NT;
-    static_assert(ROWS * L::WORDS % NT == 0, "whole words per thread");
+    static constexpr int N = ROWS * L::WORDS / NT, STEP = NT / L::WORDS;                // rows between a thread's words
+    static_assert(ROWS * L::WORDS % NT == 0 && NT % L::WORDS == 0, "whole words per thread, all in one column");
     u32x4 w[N];
+    static __device__ __forceinline__ bool inside(i32 r0, i32 rows, u32 D) { return r0 + ROWS <= rows && D == (u32)DP; }
     // rows [r0, ...) of `base`, of which those below `rows` exist (rows > 0)
     __device__ __forceinline__ void load(const T* base, u64 step, i32 r0, i32 rows, u32 D, int tid)
     {
-        const int last = (int)D / L::PER - 1;
+        if (inside(r0, rows, D) && step < (1u << 24)) {
+            const char* from = (const char*)(base + (u64)(u32)r0 * step);
+            const u32 at = ((u32)(tid / L::WORDS) * (u32)step + (u32)(tid % L::WORDS) * L::PER) * (u32)sizeof(T);
+#pragma unroll
+            for (int n = 0; n < N; ++n) w[n] = *(const u32x4*)(from + (u64)(n * STEP) * step * sizeof(T) + at);
+            return;
+        }
+        const int last = (int)D / L::PER - 1, word = tid % L::WORDS < last ? tid % L::WORDS : last;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int e = tid + n * NT, word = e % L::WORDS;
-            const i32 r = r0 + e / L::WORDS;
-            w[n] = *(const u32x4*)(base + (u64)(u32)(r < rows ? r : rows - 1) * step + (word < last ? word : last) * L::PER);
+            const i32 r = r0 + tid / L::WORDS + n * STEP;
+            w[n] = *(const u32x4*)(base + (u64)(u32)(r < rows ? r : rows - 1) * step + word * L::PER);
         }
     }
-    __device__ __forceinline__ void store(char* lds, i32 r0, i32 rows, u32 D, int tid) const
+    __device__ __forceinline__ void store(char* lds, i32 r0, i32 rows, u32 D, int tid)
     {
-        const int words = (int)D / L::PER;
+        if (!inside(r0, rows, D)) {
+            const bool on = tid % L::WORDS < (int)D / L::PER;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int e = tid + n * NT, r = e / L::WORDS, word = e % L::WORDS;
-            *(u32x4*)(lds + L::at(r, word)) = r0 + r < rows && word < words ? w[n] : u32x4{0, 0, 0, 0};
+            for (int n = 0; n < N; ++n) if (!(on & (r0 + tid / L::WORDS + n * STEP < rows))) w[n] = u32x4{0, 0, 0, 0};
         }
+#pragma unroll
+        for (int n = 0; n < N; ++n) *(u32x4*)(lds + L::at(tid / L::WORDS + n * STEP, tid % L::WORDS)) = w[n];
     }
 };
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+// the larger value, and the sum, of a lane and the lane 32 away: one instruction swaps the upper half of one register with the
+// lower half of another (the copy has to be another register, so the compiler may not see that it is one)
+struct Halves { float lo, hi; };
+__device__ __forceinline__ Halves halves(float v)
+{
+    u32 x = __builtin_bit_cast(u32, v), y = x;
+    asm("" : "+v"(y));
+    const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    x = r[0];                                                  // (a bit cast of a vector's element would always take the first)
+    y = r[1];
+    return Halves{__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)};
+}
+__device__ __forceinline__ float max_of_halves(float v) { const Halves h = halves(v); return fmaxf(h.lo, h.hi); }
+__device__ __forceinline__ float sum_of_halves(float v) { const Halves h = halves(v); return h.lo + h.hi; }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // element e of a result row: rounded once from f32

@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
 #pragma unroll
             for (int j = 0; j < 8; ++j) delta += M::at(go[c], j) * M::at(y, j);
         }
-        delta += other_half(delta);
+        delta = sum_of_halves(delta);
     }
     float lse2 = __builtin_inff();                            // exp(x - inf) = 0: a query that sees nothing has no gradient
     if (on) {

@@ -207,9 +207,9 @@ extern "C" int32_t aixk_matmul_epilogue_backward(aixk_ctx* ctx, const aixhip_ten
             wide = wide && s.p1 == 1 && (M <= 1 || s.p0 % (16 / es) == 0) && aligned16(s.pre);
         }
         if (dz) { s.dz = start(dz); wide = wide && aligned16(s.dz); }
-        // chunks of rows until every compute unit has two workgroups, none below 32 rows
+        // chunks of rows until every compute unit has four workgroups, none below 32 rows
         const u64 across = (N + (wide ? 255 : 63)) / (wide ? 256 : 64);
-        u64 chunks = ((u64)ctx->cus * 2 + across - 1) / across;
+        u64 chunks = ((u64)ctx->cus * 4 + across - 1) / across;
         if (chunks > (M + 31) / 32) chunks = (M + 31) / 32;
         if (chunks > 65535) chunks = 65535;
         if (chunks < 1) chunks = 1;
