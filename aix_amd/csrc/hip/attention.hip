@@ -46,9 +46,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    const u32 id = xcd_order(blockIdx.x, gridDim.x);
-    const u32 head = id / a.tiles, tile = a.tiles - 1 - id % a.tiles;       // longest rows of a causal mask first
-    const u32 b = head / s.H, h = head % s.H, hk = h / s.G;
+    const Place at = place_of(s, blockIdx.x, s.B * s.H);                     // (the last rows of a causal mask are the longest)
+    const u32 keys = s.B * s.HK, tile = a.tiles - 1 - at.rank;
+    const u32 b = at.head % keys / s.HK, hk = at.head % keys % s.HK, h = hk * s.G + at.head / keys;
     const Row r = row_of(s, b);
     const T* K = (const T*)a.k.p + b * a.k.b + hk * a.k.h;
     const T* V = (const T*)a.v.p + b * a.v.b + hk * a.v.h;
@@ -101,12 +101,11 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
         }
         if (!all_visible(s, r.length, r.start + w0, r.start + w1, j0, j0 + KT - 1)) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb) {
+                const u32 word = seen.word(j0 + kb * 32) >> (4 * half);
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const i32 j = j0 + kb * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
-                    x[kb][v] = seen(j) ? x[kb][v] : -__builtin_inff();
-                }
+                for (int v = 0; v < 16; ++v) x[kb][v] = hide(x[kb][v], word, 8 * (v >> 2) + (v & 3));
+            }
         }
         float top = x[0][0];
 #pragma unroll
@@ -169,9 +168,9 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 512 ? 2 : 1) void attention1
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c15 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    const u32 id = xcd_order(blockIdx.x, gridDim.x);
-    const u32 head = id / a.tiles, tile = a.tiles - 1 - id % a.tiles;
-    const u32 b = head / s.H, h = head % s.H, hk = h / s.G;
+    const Place at = place_of(s, blockIdx.x, s.B * s.H);                     // (the last rows of a causal mask are the longest)
+    const u32 keys = s.B * s.HK, tile = a.tiles - 1 - at.rank;
+    const u32 b = at.head % keys / s.HK, hk = at.head % keys % s.HK, h = hk * s.G + at.head / keys;
     const Row r = row_of(s, b);
     const T* K = (const T*)a.k.p + b * a.k.b + hk * a.k.h;
     const T* V = (const T*)a.v.p + b * a.v.b + hk * a.v.h;
@@ -223,14 +222,19 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 512 ? 2 : 1) void attention1
             for (int k = 0; k < SUB; ++k) x[k] = M::run16(L::row(ks, k * 16 + c15, 4 * c + g), q[c], x[k]);
         }
         const bool masked = !all_visible(s, r.length, r.start + w0, r.start + w1, j0, j0 + KT - 1);
+        if (masked) {
+#pragma unroll
+            for (int k = 0; k < SUB; k += 2) {
+                const u32 word = seen.word(j0 + k * 16) >> (4 * g);
+#pragma unroll
+                for (int v = 0; v < 8; ++v) x[k + (v >> 2)][v & 3] = hide(x[k + (v >> 2)][v & 3], word, 16 * (v >> 2) + (v & 3));
+            }
+        }
         float top = -__builtin_inff();
 #pragma unroll
         for (int k = 0; k < SUB; ++k)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                if (masked) x[k][v] = seen(j0 + k * 16 + 4 * g + v) ? x[k][v] : -__builtin_inff();
-                top = fmaxf(top, x[k][v]);
-            }
+            for (int v = 0; v < 4; ++v) top = fmaxf(top, x[k][v]);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = max_of_halves(top) * c2;
         if (__any(top > m + 8.0f)) {
@@ -390,11 +394,12 @@ __global__ __launch_bounds__(WAVES * 64) void attention_split_k(SplitArgs a)
         if (n + WAVES < to) load(tile_at(t, n + WAVES) * KT);
 
         float top = -__builtin_inff();
+        const u32 word = seen.word(j0) >> (4 * g);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                x[kb][v] = seen(j0 + kb * 16 + 4 * g + v) ? x[kb][v] * c2 : -__builtin_inff();
+                x[kb][v] = hide(x[kb][v] * c2, word, 16 * kb + v);
                 top = fmaxf(top, x[kb][v]);
             }
         top = fmaxf(top, __shfl_xor(top, 16, 64));

@@ -52,39 +52,50 @@ __device__ __forceinline__ Row row_of(const Shape& s, u32 b)
     return r;
 }
 
-// The keys the query at position p sees: lo <= j < lo + n, and j < sink.  Three comparisons per key without a branch (the mask's
-// definition written out per element becomes a branch per condition and element).
+// Masks as words of 32 bits, one bit per key (per query): formed once for 32 elements, then two instructions per element -- the
+// bit as a word of ones or zeros, and a select or an and -- where the definition's comparisons take five and, written out per
+// element, a branch per condition.
+__device__ __forceinline__ u32 ones_below(i32 n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ u32 spread(u32 word, int bit) { return (u32)((i32)(word << (31 - bit)) >> 31); }
+__device__ __forceinline__ float hide(float x, u32 word, int bit)         // -infinity where the bit is not set
+{
+    const u32 t = spread(word, bit);
+    return __builtin_bit_cast(float, (__builtin_bit_cast(u32, x) & t) | (0xFF800000u & ~t));
+}
+__device__ __forceinline__ float drop(float x, u32 word, int bit) { return __builtin_bit_cast(float, __builtin_bit_cast(u32, x) & spread(word, bit)); }
+
+// The keys the query at position p sees: lo <= j < hi, and j < sink.
 struct Keys {
-    i32 lo; u32 n; i32 sink;
-    __device__ __forceinline__ bool operator()(i32 j) const { return ((u32)(j - lo) < n) | (j < sink); }
+    i32 lo, hi, sink;
+    // keys j0 .. j0 + 31
+    __device__ __forceinline__ u32 word(i32 j0) const { return (ones_below(hi - j0) & ~ones_below(lo - j0)) | ones_below(sink - j0); }
 };
 __device__ __forceinline__ Keys keys_of(const Shape& s, i32 length, i32 p)
 {
-    i32 hi = length, lo = 0;                                  // [lo, hi)
-    if (s.causal && p + 1 < hi) hi = p + 1;
-    Keys k{0, 0u, 0};
+    Keys k{0, 0, 0};
     if (p < 0) return k;
+    i32 hi = length;
+    if (s.causal && p + 1 < hi) hi = p + 1;
     if (s.window) {
         k.sink = s.sinks < hi ? s.sinks : hi;
         if ((i64)p + s.window < hi) hi = p + s.window;
-        if (p >= s.window) lo = p - s.window + 1;
+        if (p >= s.window) k.lo = p - s.window + 1;
     }
-    k.lo = lo;
-    k.n = hi > lo ? (u32)(hi - lo) : 0u;
+    k.hi = hi;
     return k;
 }
-// The positions that see key j, lo <= p < lo + n.
+// The positions that see key j: lo <= p < hi.
 struct Queries {
-    i32 lo; u32 n;
-    __device__ __forceinline__ bool operator()(i32 p) const { return (u32)(p - lo) < n; }
+    i32 lo, hi;
+    __device__ __forceinline__ u32 word(i32 p0) const { return ones_below(hi - p0) & ~ones_below(lo - p0); }
 };
 __device__ __forceinline__ Queries queries_of(const Shape& s, i32 length, i32 j)
 {
-    if (j >= length) return Queries{0, 0u};
+    if (j >= length) return Queries{0, 0};
     const bool near = s.window && j >= s.sinks;
     const i32 lo = s.causal ? j : near && j >= s.window ? j - s.window + 1 : 0;
-    const i64 hi = near && (i64)j + s.window < 0x7FFFFFFF ? (i64)j + s.window : 0x7FFFFFFF;
-    return Queries{lo, (u32)(hi - lo)};
+    constexpr i32 kEnd = 0x50000000;                           // behind every position (2^30), and within 32 bits of the first (-2^29)
+    return Queries{lo, near && (i64)j + s.window < kEnd ? j + s.window : kEnd};
 }
 // every / no pair of the rows at positions [p0, p1] and the keys [j0, j1] is visible
 __device__ __forceinline__ bool all_visible(const Shape& s, i32 length, i32 p0, i32 p1, i32 j0, i32 j1)
@@ -130,6 +141,20 @@ __device__ __forceinline__ u32 xcd_order(u32 id, u32 n)
 {
     const u32 q = n / 8u, r = n % 8u, x = id % 8u;
     return x * q + (x < r ? x : r) + id / 8u;
+}
+
+// A grid of `heads` x ranks: workgroup id stands for the (id / heads)-th rank -- the heaviest first -- of head id % heads.  Ids go
+// round the XCDs, so with a multiple of eight key heads a key head and all query heads on it stay on one XCD, whose L2 then
+// holds its keys, and every XCD gets every rank.  Sequences of different lengths are moved on by one from rank to rank: the long
+// ones do not stay on the XCDs of their heads (777 padded f32, of four sequences: 43.4 -> PADDED_US us).
+struct Place { u32 rank, head; };
+__device__ __forceinline__ Place place_of(const Shape& s, u32 id, u32 heads)
+{
+    Place p;
+    p.rank = id / heads;
+    p.head = id % heads;
+    if (s.lengths) p.head = (p.head + p.rank) % heads;
+    return p;
 }
 
 // ---- matrix instructions over fragments of eight elements ------------------------------------------------------------
@@ -264,12 +289,12 @@ template <class T, int DP> struct Tile {
 // ROWS rows of DP elements on their way from memory into such a tile through the registers of NT threads.  A tile whose rows
 // all exist and whose rows are DP elements is fetched from a uniform address and one offset per thread; at an edge the
 // addresses stay inside the operand and zeros are chosen when the words are stored.
-template <class T, int DP, int ROWS, int NT> struct Stage {
+template <class T, int DP, int ROWS, int NT, bool WHOLE = true> struct Stage {
     typedef Tile<T, DP> L;
     static constexpr int N = ROWS * L::WORDS / NT, STEP = NT / L::WORDS;                // rows between a thread's words
     static_assert(ROWS * L::WORDS % NT == 0 && NT % L::WORDS == 0, "whole words per thread, all in one column");
     u32x4 w[N];
-    static __device__ __forceinline__ bool inside(i32 r0, i32 rows, u32 D) { return r0 + ROWS <= rows && D == (u32)DP; }
+    static __device__ __forceinline__ bool inside(i32 r0, i32 rows, u32 D) { return WHOLE && r0 + ROWS <= rows && D == (u32)DP; }
     // rows [r0, ...) of `base`, of which those below `rows` exist (rows > 0)
     __device__ __forceinline__ void load(const T* base, u64 step, i32 r0, i32 rows, u32 D, int tid)
     {

@@ -45,9 +45,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    const u32 id = xcd_order(blockIdx.x, gridDim.x);
-    const u32 head = id / a.tiles, tile = a.tiles - 1 - id % a.tiles;
-    const u32 b = head / s.H, h = head % s.H, hk = h / s.G;
+    const Place place = place_of(s, blockIdx.x, s.B * s.H);
+    const u32 keys = s.B * s.HK, tile = a.tiles - 1 - place.rank;
+    const u32 b = place.head % keys / s.HK, hk = place.head % keys % s.HK, h = hk * s.G + place.head / keys;
     const Row r = row_of(s, b);
     const T* K = (const T*)a.k.p + b * a.k.b + hk * a.k.h;
     const T* V = (const T*)a.v.p + b * a.v.b + hk * a.v.h;
@@ -123,8 +123,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
                 e[v] = exp2_of(x[v] * c2 - lse2) * (dp[v] - delta);
             }
             if (masked) {
+                const u32 word = seen.word(k0) >> (4 * half);
 #pragma unroll
-                for (int v = 0; v < 16; ++v) e[v] = seen(k0 + 8 * (v >> 2) + 4 * half + (v & 3)) ? e[v] : 0.0f;
+                for (int v = 0; v < 16; ++v) e[v] = drop(e[v], word, 8 * (v >> 2) + (v & 3));
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -191,8 +192,8 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
     // a head's workgroups: the lead tiles with lead_splits shares each, then the others with `splits`
-    const u32 per_head = a.lead * a.lead_splits + (a.tiles - a.lead) * a.splits;
-    const u32 id = xcd_order(blockIdx.x, gridDim.x), head = id / per_head, in = id % per_head;
+    const Place place = place_of(s, blockIdx.x, s.B * s.HK);
+    const u32 head = place.head, in = place.rank;
     const bool leads = in < a.lead * a.lead_splits;
     const u32 splits = leads ? a.lead_splits : a.splits, in2 = leads ? in : in - a.lead * a.lead_splits;
     const u32 split = in2 % splits, tile = in2 / splits + (leads ? 0 : a.lead);
@@ -256,7 +257,7 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
     // the (head of the group, tile) of a step, stepped on by counting (a division per step costs more than its products)
     struct At { u32 g; i32 tile; };
     auto on_from = [&](At& at) { if (++at.tile == per) { at.tile = 0; ++at.g; } };
-    Stage<T, DP, QT, NT> sq, sg;
+    Stage<T, DP, QT, NT, !KL> sq, sg;                       // (with the keys in LDS the second way to fetch costs registers there are not)
     float next_l = 0.0f, next_d = 0.0f;
     auto load = [&](const At& at) {
         const u32 h = hk * s.G + at.g;
@@ -304,11 +305,11 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
                 }
             }
             if (masked) {
+                const u32 word = seen.word(r.start + q0) >> (4 * half);
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    const bool ok = seen(r.start + q0 + 8 * (v >> 2) + 4 * half + (v & 3));
-                    e[v] = ok ? e[v] : 0.0f;
-                    w[v] = ok ? w[v] : 0.0f;
+                    e[v] = drop(e[v], word, 8 * (v >> 2) + (v & 3));
+                    w[v] = drop(w[v], word, 8 * (v >> 2) + (v & 3));
                 }
             }
 #pragma unroll
