@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
     typedef Mma<T> M;
     typedef typename M::Frag Frag;
     typedef Tile<T, DP> L;
-    constexpr int KT = 64, DB = DP / 32, DC = DP / 16;
+    constexpr int KT = DP <= 128 ? 64 : 32, KB = KT / 32, DB = DP / 32, DC = DP / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     char* ks = lds;
     char* vs = lds + KT * L::PITCH;
@@ -92,16 +92,16 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
         }
         if (w0 > w1 || none_visible(s, r.length, r.start + w0, r.start + w1, j0, j0 + KT - 1)) continue;
 
-        f32x16 x[2];
+        f32x16 x[KB];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < KB; ++kb) {
             x[kb] = f32x16{};
 #pragma unroll
             for (int c = 0; c < DC; ++c) if (!past<T, DP>(c * 16, s.DW)) x[kb] = M::run32(L::row(ks, kb * 32 + (lane & 31), 2 * c + half), q[c], x[kb]);
         }
         if (!all_visible(s, r.length, r.start + w0, r.start + w1, j0, j0 + KT - 1)) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
+            for (int kb = 0; kb < KB; ++kb) {
                 const u32 word = seen.word(j0 + kb * 32) >> (4 * half);
 #pragma unroll
                 for (int v = 0; v < 16; ++v) x[kb][v] = hide(x[kb][v], word, 8 * (v >> 2) + (v & 3));
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
         }
         float top = x[0][0];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int v = 0; v < 16; ++v) top = fmaxf(top, x[kb][v]);
         top = max_of_halves(top) * c2;
@@ -124,9 +124,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
                 for (int v = 0; v < 16; ++v) o[d][v] *= keep;
         }
         const float ref = m == -__builtin_inff() ? 0.0f : m;   // a row without a visible key so far: every term is exp(-inf)
-        Frag w[4];
+        Frag w[2 * KB];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < KB; ++kb) {
             float e[16];
 #pragma unroll
             for (int v = 0; v < 16; ++v) { e[v] = exp2_of(x[kb][v] * c2 - ref); l += e[v]; }
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
             w[2 * kb + 1] = M::pack8(e + 8);
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2 * KB; ++c)
 #pragma unroll
             for (int d = 0; d < DB; ++d) if (!past<T, DP>(d * 32, s.DW)) o[d] = M::run32(L::column(vs, c * 16, d, lane), w[c], o[d]);
     }
@@ -521,14 +521,50 @@ __global__ __launch_bounds__(256) void attention_join_k(SplitArgs a)
 }
 
 // ---- operands the kernels cannot read where they lie ----------------------------------------------------------------------
-// [batch, heads, sequence, D] through any strides into dense rows of DW elements (whole 16-byte words), zeros behind D.
+// [batch, heads, rows, D] through any strides into dense rows of DW elements (whole 16-byte words), zeros behind D.  A group of
+// `lanes` lanes takes a row, a word per lane and turn, so the row's place is worked out once per row.
 template <class T>
-__global__ __launch_bounds__(256) void attention_pack_k(View src, T* dst, u32 H, u64 S, u32 D, u32 DW, u64 total)
+__global__ __launch_bounds__(256) void attention_pack_k(View src, T* dst, u32 H, u32 S, u32 D, u32 DW, u64 rows, u32 lanes)
 {
-    for (u64 e = (u64)blockIdx.x * 256 + threadIdx.x; e < total; e += (u64)gridDim.x * 256) {
-        const u32 d = (u32)(e % DW);
-        const u64 row = e / DW, i = row % S, bh = row / S, h = bh % H, b = bh / H;
-        dst[e] = d < D ? ((const T*)src.p)[b * src.b + h * src.h + i * src.s + d * src.d] : zero<T>();
+    constexpr u32 PER = 16 / sizeof(T);
+    const u32 lane = threadIdx.x % lanes, each = 256 / lanes;
+    for (u64 row = (u64)blockIdx.x * each + threadIdx.x / lanes; row < rows; row += (u64)gridDim.x * each) {
+        const u32 i = (u32)(row % S), bh = (u32)(row / S), h = bh % H, b = bh / H;
+        const T* from = (const T*)src.p + b * src.b + h * src.h + i * src.s;
+        T* to = dst + row * DW;
+        for (u32 w = lane; w < DW / PER; w += lanes) {
+            union { u32x4 word; T x[PER]; } v;
+            if (src.d == 1 && w * PER + PER <= D) __builtin_memcpy(&v, from + w * PER, 16);        // (any alignment)
+            else
+#pragma unroll
+            for (u32 j = 0; j < PER; ++j) { const u32 d = w * PER + j; v.x[j] = d < D ? from[(u64)d * src.d] : zero<T>(); }
+            *(u32x4*)(to + w * PER) = v.word;
+        }
+    }
+}
+
+// The same for rows that lie side by side (unit stride from row to row): 64 x 64 elements at a time turned in LDS, so that both
+// the loads and the stores are of whole lines.
+template <class T>
+__global__ __launch_bounds__(256) void attention_pack_turned_k(View src, T* dst, u32 H, u32 S, u32 D, u32 DW, u32 across, u32 down, u64 tiles)
+{
+    constexpr u32 PER = 16 / sizeof(T), WORDS = 64 / PER;
+    __shared__ T tile[64][64 + 4 / sizeof(T)];
+    for (u64 at = blockIdx.x; at < tiles; at += gridDim.x) {
+        const u32 tx = (u32)(at % across), ty = (u32)(at / across % down), bh = (u32)(at / across / down), h = bh % H, b = bh / H;
+        const u32 s0 = ty * 64, d0 = tx * 64, lane = threadIdx.x & 63;
+        const T* from = (const T*)src.p + b * src.b + h * src.h + s0 + lane;
+        for (u32 d = threadIdx.x >> 6; d < 64; d += 4) tile[d][lane] = s0 + lane < S && d0 + d < D ? from[(u64)(d0 + d) * src.d] : zero<T>();
+        __syncthreads();
+        for (u32 c = threadIdx.x; c < 64 * WORDS; c += 256) {
+            const u32 r = c / WORDS, w = c % WORDS;
+            if (s0 + r >= S || d0 + w * PER >= DW) continue;
+            union { u32x4 word; T x[PER]; } v;
+#pragma unroll
+            for (u32 j = 0; j < PER; ++j) v.x[j] = tile[w * PER + j][r];
+            *(u32x4*)(dst + ((u64)bh * S + s0 + r) * DW + d0 + w * PER) = v.word;
+        }
+        __syncthreads();
     }
 }
 
@@ -539,14 +575,23 @@ namespace attn {
 
 int pack(aixk_ctx* ctx, int dtype, const View& src, void* dst, u32 B, u32 H, u64 S, u32 D, u32 DW)
 {
-    const u64 total = (u64)B * H * S * DW;
-    if (!total) return AIXK_OK;
-    const unsigned blocks = grid_for(total, 256, (unsigned)ctx->cus * 16u);
-    if (dtype == AIXK_F32) hipLaunchKernelGGL((attention_pack_k<float>), dim3(blocks), dim3(256), 0, ctx->stream, src, (float*)dst, H, S, D, DW, total);
-    else if (dtype == AIXK_F16) hipLaunchKernelGGL((attention_pack_k<f16>), dim3(blocks), dim3(256), 0, ctx->stream, src, (f16*)dst, H, S, D, DW, total);
-    else hipLaunchKernelGGL((attention_pack_k<bf16>), dim3(blocks), dim3(256), 0, ctx->stream, src, (bf16*)dst, H, S, D, DW, total);
-    AIXK_HIP(hipGetLastError());
-    return AIXK_OK;
+    const u64 rows = (u64)B * H * S;
+    if (!rows || !DW) return AIXK_OK;
+    AIXK_REQUIRE(S < (1ull << 32) && (u64)B * H < (1ull << 32), "operand copy: shape too large");
+    const u32 words = DW / (16 / (u32)aixk_dtype_size(dtype));
+    u32 lanes = 1;
+    while (lanes < words && lanes < 64) lanes *= 2;
+    const unsigned blocks = grid_for((rows * lanes + 255) / 256, 1, (unsigned)ctx->cus * 16u);
+    const u32 across = (DW + 63) / 64, down = (u32)((S + 63) / 64);
+    const u64 tiles = (u64)across * down * B * H;
+    auto run = [&](auto type) -> int {
+        typedef decltype(type) T;
+        if (src.s == 1 && src.d != 1 && S > 1 && D > 1) hipLaunchKernelGGL((attention_pack_turned_k<T>), dim3(grid_for(tiles, 1, (unsigned)ctx->cus * 16u)), dim3(256), 0, ctx->stream, src, (T*)dst, H, (u32)S, D, DW, across, down, tiles);
+        else hipLaunchKernelGGL((attention_pack_k<T>), dim3(blocks), dim3(256), 0, ctx->stream, src, (T*)dst, H, (u32)S, D, DW, rows, lanes);
+        AIXK_HIP(hipGetLastError());
+        return AIXK_OK;
+    };
+    return dtype == AIXK_F32 ? run(float{}) : dtype == AIXK_F16 ? run(f16{}) : run(bf16{});
 }
 
 namespace {
@@ -572,7 +617,7 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
         AIXK_REQUIRE(wide < (1ull << 31), "attention: too many rows");
         if constexpr (sizeof(T) == 2) {
         ForwardArgs a{s, c.q, c.k, c.v, c.out, c.lse, ((u32)s.SQ + 127) / 128, c.whole_out};
-        constexpr size_t lds = 2 * 64 * DP * sizeof(T);
+        constexpr size_t lds = 2 * (DP <= 128 ? 64 : 32) * DP * sizeof(T);
         AIXK_TRY(allow_lds(attention_k<T, DP>, lds));
         hipLaunchKernelGGL((attention_k<T, DP>), dim3((unsigned)wide), dim3(256), lds, ctx->stream, a);
         AIXK_HIP(hipGetLastError());

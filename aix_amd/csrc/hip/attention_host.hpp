@@ -10,7 +10,7 @@ namespace aixk {
 namespace attn {
 
 // slots of the context's scratch memory (block_scratch)
-enum { kScratchQ = 0, kScratchK, kScratchV, kScratchGrad, kScratchOut, kScratchParts, kScratchDelta, kScratchProduct, kScratchColumns };
+enum { kScratchQ = 0, kScratchK, kScratchV, kScratchGrad, kScratchOut, kScratchParts, kScratchDelta, kScratchProduct, kScratchColumns, kScratchLeft, kScratchRight };
 
 int pack(aixk_ctx* ctx, int dtype, const View& src, void* dst, u32 B, u32 H, u64 S, u32 D, u32 DW);      // attention.hip
 

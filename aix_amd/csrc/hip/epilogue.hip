@@ -10,6 +10,7 @@ using namespace aixk;
 
 namespace aixk {
 int matmul_mfma_epilogue(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const EpiArgs& epi);      // matmul_mfma.hip
+int matmul_plain(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out);
 }
 
 namespace {
@@ -239,11 +240,11 @@ extern "C" int32_t aixk_matmul_epilogue_backward(aixk_ctx* ctx, const aixhip_ten
     const aixhip_tensor* z = dz ? dz : grad;
     if (da && M && K) {
         const aixhip_tensor bt = transposed(b), o = from_start(da);
-        AIXK_TRY(aixk_matmul(ctx, z, &bt, &o));
+        AIXK_TRY(matmul_plain(ctx, z, &bt, &o));
     }
     if (db && K && N) {
         const aixhip_tensor at = transposed(a), o = from_start(db);
-        AIXK_TRY(aixk_matmul(ctx, &at, z, &o));
+        AIXK_TRY(matmul_plain(ctx, &at, z, &o));
     }
     return AIXK_OK;
 }

@@ -46,6 +46,7 @@ using namespace aixk;
 
 namespace aixk {
 int gather_dense(aixk_ctx* ctx, const aixhip_tensor* src, void* dst, uint64_t n);     // layout.hip
+int matmul_mfma_epilogue(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, const EpiArgs& epi);
 int matmul_rows(aixk_ctx* ctx, int dtype, const void* a, u64 lda, const void* b, u64 ldb, bool bt, void* out, u64 M, u64 N, u64 K, const EpiArgs& epi, u32* shares, float** partial);      // matmul_rows.hip
 }
 
@@ -2355,6 +2356,34 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
     return AIXK_OK;
 }
 
+// A product that nothing follows, for the operators of transformer blocks: aixk_matmul's own kernels where they take the shape.
+// What would be left to its LDS-tiled kernel -- contractions without whole 16-byte words (the rows of a batch in a weight
+// gradient), results below 64 x 64 elements -- has its operands copied K-contiguous with zeros up to a whole word.
+// (f32 [1216, 11127] x [11127, 128] XODD_US; f32 [1, 2624] x [2624, 64] XTINY_US.)
+int matmul_plain(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out)
+{
+    const uint64_t M = a->shape[0], K = a->shape[1], N = b->shape[1];
+    const size_t esz = aixk_dtype_size(out->dtype);
+    const uint64_t word = 16 / esz, Kp = (K + word - 1) / word * word;
+    if (K == 0 || (K == Kp && M * N >= 64 * 64)) return aixk_matmul(ctx, a, b, out);
+    EpiArgs nothing{};
+    nothing.whole = N % 8 == 0 && aligned16(out->data);
+    if (esz == 2) return matmul_mfma_epilogue(ctx, a, b, out, nothing);
+    aixhip_tensor ta = *a, tb = *b;
+    if (K != Kp) {
+        AIXK_REQUIRE(Kp < (1ull << 31), "matmul: shape too large");
+        void *wa, *wb;
+        AIXK_TRY(block_scratch(ctx, attn::kScratchLeft, M * Kp * esz, &wa));
+        AIXK_TRY(block_scratch(ctx, attn::kScratchRight, N * Kp * esz, &wb));
+        AIXK_TRY(attn::pack(ctx, out->dtype, attn::View{(char*)a->data + a->offset * esz, 0, 0, a->strides[0], a->strides[1]}, wa, 1, 1, M, (u32)K, (u32)Kp));
+        AIXK_TRY(attn::pack(ctx, out->dtype, attn::View{(char*)b->data + b->offset * esz, 0, 0, b->strides[1], b->strides[0]}, wb, 1, 1, N, (u32)K, (u32)Kp));
+        ta.data = wa; ta.offset = 0; ta.strides[0] = Kp; ta.strides[1] = 1; ta.shape[1] = Kp;
+        tb.data = wb; tb.offset = 0; tb.strides[0] = 1; tb.strides[1] = Kp; tb.shape[0] = Kp;
+    }
+    const int rc = matmul_mfma(ctx, &ta, &tb, out, &nothing);
+    return rc == -1 ? fail(AIXK_EINVAL, "matmul: no kernel takes these operands") : rc;
+}
+
 // A product with an epilogue.  16-bit operands: the kernels above finish their accumulators in place; A comes K-contiguous
 // and both with whole 16-byte words along K, anything else is copied first.  f32: the product as aixk_matmul forms it, then
 // one pass over the result.
@@ -2369,7 +2398,7 @@ int matmul_mfma_epilogue(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_ten
             AIXK_TRY(block_scratch(ctx, attn::kScratchProduct, (size_t)(M * N) * sizeof(float), &ws));
             product.data = ws;
         }
-        AIXK_TRY(aixk_matmul(ctx, a, b, &product));
+        AIXK_TRY(matmul_plain(ctx, a, b, &product));
         return launch_epilogue(ctx, (const float*)product.data, out, 1, epi);
     }
     constexpr size_t esz = 2;

@@ -212,9 +212,9 @@ def test_replays_of_a_captured_step_on_blocks_equal_the_eager_steps(dev):
 class Serving:
     """A single-token step on a context: rotary positions in place, attention over a cache, an output product."""
 
-    def __init__(self, gpu, batch, keys, seed):
+    def __init__(self, gpu, batch, keys, seed, window=300):
         rng = np.random.default_rng(seed)
-        self.gpu, self.b, self.keys, self.h, self.hk, self.d = gpu, batch, keys, 8, 2, 64
+        self.gpu, self.b, self.keys, self.h, self.hk, self.d, self.window = gpu, batch, keys, 8, 2, 64, window
         b, h, hk, d, e = batch, self.h, self.hk, self.d, self.h * self.d
         mk = lambda *shape: box(gpu, O.BF16, shape, rng.standard_normal(shape))      # noqa: E731
         self.q0 = mk(b, h, 1, d)
@@ -223,7 +223,7 @@ class Serving:
         self.pos, self.lengths = box(gpu, O.I32, (b, 1)), box(gpu, O.I32, (b,))
         self.w, self.bias, self.out = mk(e, 96), mk(96), box(gpu, O.BF16, (b, 96))
         self.turn = K.RotarySpec(dims=d, base=1e4, factor=1.0, original_length=1.0, low_turns=1.0, high_turns=2.0, magnitude=1.0)
-        self.spec = K.AttentionSpec(scale=0.125, causal=1, window=300, sinks=4, lengths=ptr(self.lengths), starts=None)
+        self.spec = K.AttentionSpec(scale=0.125, causal=1, window=window, sinks=4, lengths=ptr(self.lengths), starts=None)
         self.epi = K.Epilogue(bias=ptr(self.bias), residual=None, pre=None, activation=K.ACT_GELU)
         self.flat = K.tensor(self.mixed.ptr, K.BF16, (b, e))
 
@@ -242,7 +242,7 @@ class Serving:
         pos = (self.lens - 1).reshape(-1, 1)
         want, far = R.rotary(self.q0.values(), pos, self.d, 0, 0, R.frequencies(self.d), 1.0, O.BF16)
         R.check(self.q.fetch(), want, far, what + " turn")
-        seen = R.visible(self.b, 1, self.keys, True, 300, 4, self.lens, None)
+        seen = R.visible(self.b, 1, self.keys, True, self.window, 4, self.lens, None)
         out, _, far, _ = R.attention(self.q.fetch(), self.k.values(), self.v.values(), seen, 0.125, O.BF16)
         R.check(self.mixed.fetch(), out, far, what + " attention")
         want, far, _, _ = R.matmul_epilogue(self.mixed.fetch().reshape(self.b, -1), self.w.values(), self.bias.values(), None, "gelu", O.BF16)
@@ -265,7 +265,7 @@ def test_two_captured_serving_steps_share_their_context(dev):
             g = C.c_void_p()
             gpu.ctx.call("aixk_capture_end", C.byref(g))
             graphs.append(g)
-        big = Serving(gpu, 40, 3000, 3)                       # partial results of more rows than either captured step had
+        big = Serving(gpu, 40, 3000, 3, window=2000)          # partial results of more rows than either captured step had
         big.at(np.linspace(1, 3000, 40).astype(int))
         big.step()
         big.check("eager, larger")
@@ -290,7 +290,7 @@ def test_two_captured_serving_steps_share_their_context(dev):
 def test_outgrown_workspaces_inside_a_capture_are_refused(dev):
     gpu = G.Gpu()
     try:
-        s = Serving(gpu, 40, 3000, 3)
+        s = Serving(gpu, 40, 3000, 3, window=2000)            # (a window of 300 is one workgroup's work and needs no workspace)
         s.at([3000] * 40)
         gpu.ctx.call("aixk_capture_begin")
         rc = gpu.ctx.lib.aixk_attention(gpu.ctx.handle, ref(s.q0), ref(s.k), ref(s.v), C.byref(s.spec), ref(s.mixed), None)
