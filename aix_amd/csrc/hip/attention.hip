@@ -344,8 +344,20 @@ __global__ __launch_bounds__(WAVES * 64) void attention_split_k(SplitArgs a)
     // slot of 16-byte word c of key k in the slab: the transposed reads take 32 bytes from each of eight keys at a time
     auto turn = [](int k) { return WORDS >= 16 ? ((k & 7) << 1) | ((k >> 3) & 1) : ((k >> 1) & 3) << 1; };
     const int last = (int)s.DW / PER - 1;
+    // rows of 1 KB: the registers hold no next step beside this one.  Keys and values come within their step, V in two turns (a
+    // step of the four waves is 256 KB, several times what a compute unit's share of the bandwidth brings in the time of a load)
+    constexpr bool LATE = DP * sizeof(T) > 512;
+    constexpr int TURNS = LATE ? 2 : 1, NW = NV / TURNS;
     Frag kf[2][DC];
-    u32x4 vf[NV];
+    u32x4 vf[NW];
+    auto load_v = [&](i32 j0, int turn) {
+#pragma unroll
+        for (int n = 0; n < NW; ++n) {
+            const int e = lane + (turn * NW + n) * 64, w = e % WORDS;
+            const i32 j = j0 + e / WORDS;
+            vf[n] = *(const u32x4*)(V + (u64)(u32)(j < r.length ? j : r.length - 1) * a.v.s + (w < last ? w : last) * PER);
+        }
+    };
     auto load = [&](i32 j0) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -361,17 +373,13 @@ __global__ __launch_bounds__(WAVES * 64) void attention_split_k(SplitArgs a)
                 }
             }
         }
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int e = lane + n * 64, w = e % WORDS;
-            const i32 j = j0 + e / WORDS;
-            vf[n] = *(const u32x4*)(V + (u64)(u32)(j < r.length ? j : r.length - 1) * a.v.s + (w < last ? w : last) * PER);
-        }
+        if constexpr (!LATE) load_v(j0, 0);
     };
     i32 n = from + wave;
-    if (n < to) load(tile_at(t, n) * KT);
+    if (!LATE && n < to) load(tile_at(t, n) * KT);
     for (; n < to; n += WAVES) {
         const i32 j0 = tile_at(t, n) * KT;
+        if constexpr (LATE) load(j0);
         f32x4 x[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -387,11 +395,15 @@ __global__ __launch_bounds__(WAVES * 64) void attention_split_k(SplitArgs a)
             }
         }
 #pragma unroll
-        for (int e = 0; e < NV; ++e) {
-            const int at = lane + e * 64, k = at / WORDS, w = at % WORDS;
-            *(u32x4*)(slab + k * PITCH + ((w ^ turn(k)) << 4)) = j0 + k < r.length && w <= last ? vf[e] : u32x4{0, 0, 0, 0};
+        for (int u = 0; u < TURNS; ++u) {
+            if constexpr (LATE) load_v(j0, u);
+#pragma unroll
+            for (int e = 0; e < NW; ++e) {
+                const int at = lane + (u * NW + e) * 64, k = at / WORDS, w = at % WORDS;
+                *(u32x4*)(slab + k * PITCH + ((w ^ turn(k)) << 4)) = j0 + k < r.length && w <= last ? vf[e] : u32x4{0, 0, 0, 0};
+            }
         }
-        if (n + WAVES < to) load(tile_at(t, n + WAVES) * KT);
+        if (!LATE && n + WAVES < to) load(tile_at(t, n + WAVES) * KT);
 
         float top = -__builtin_inff();
         const u32 word = seen.word(j0) >> (4 * g);
@@ -645,7 +657,8 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
     // eight workgroups where a share still has eight steps (16 sequences of any length up to 32768: 193 us with shares for four
     // workgroups, 172 for eight, which even the lengths out; 2052 keys: 31.0 us with four, 34.2 with eight).
     const u64 steps = (keys + kSplitKeys * 4 - 1) / (kSplitKeys * 4);
-    u64 splits = ((u64)ctx->cus * 4 + narrow - 1) / narrow;
+    constexpr u64 resident = 163840 / SplitLds<T, DP, 4>::kBytes < 4 ? 163840 / SplitLds<T, DP, 4>::kBytes : 4;
+    u64 splits = ((u64)ctx->cus * resident + narrow - 1) / narrow;
     splits = std::max<u64>(splits, std::min<u64>(((u64)ctx->cus * 8 + narrow - 1) / narrow, steps / 8));
     if (splits > steps) splits = steps;
     if (splits < 1) splits = 1;

@@ -80,9 +80,11 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
         if (saved != -__builtin_inff()) lse2 = saved * kLog2e;
         if (half == 0) a.delta[at] = delta;
     }
-    f32x16 acc[DB];
+    f32x16 acc[DB], less;                                     // (grad v^T starts from -delta: the products subtract it)
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
+#pragma unroll
+    for (int v = 0; v < 16; ++v) less[v] = -delta;
     const float c2 = s.scale * kLog2e;
 
     const Keys seen = keys_of(s, r.length, p);
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
         for (int kb = 0; kb < KT / 32; ++kb) {
             const i32 k0 = j0 + kb * 32;
             if (none_visible(s, r.length, r.start + w0, r.start + w1, k0, k0 + 31)) continue;
-            f32x16 x = f32x16{}, dp = f32x16{};
+            f32x16 x = f32x16{}, dp = less;
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
                 if (past<T, DP>(c * 16, s.DW)) break;
@@ -120,7 +122,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
             float e[16];
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-                e[v] = exp2_of(x[v] * c2 - lse2) * (dp[v] - delta);
+                e[v] = exp2_of(x[v] * c2 - lse2) * dp[v];
             }
             if (masked) {
                 const u32 word = seen.word(k0) >> (4 * half);
@@ -147,13 +149,14 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
 // A wave keeps both sums of its 32 keys in registers, and the keys and values where the registers hold them beside that.  Rows of
 // 256 bytes: sums of 128 registers leave room for two waves per SIMD only with keys and values in LDS (32 more registers for the
 // keys alone cost eight spilled ones and 18 %: each reload waits for the loads in flight), 144 KB for eight waves; one wave
-// per SIMD with everything in registers takes 1.4 times as long.  The queries and gradients of every head of the group come by in tiles of QT rows.  Here a lane is one key: P and
+// per SIMD with everything in registers takes 1.4 times as long.  Rows of 128 bytes: keys and values in LDS make room for a third
+// wave per SIMD (16 x 12 heads of 512 x 64, window 128: 28.2 us, with them in registers and two waves 32.6).  The queries and gradients of every head of the group come by in tiles of QT rows.  Here a lane is one key: P and
 // dS, rounded, feed dv^T = grad^T P and dk^T = q^T dS as they lie.
 template <class T, int DP> struct KeyBlock {
     static constexpr size_t kRow = DP * sizeof(T);
     static constexpr int kThreads = kRow == 256 ? 512 : 256, kKeys = kThreads / 2;
-    static constexpr int kWaves = kRow <= 256 ? 2 : 1;                                   // per SIMD
-    static constexpr bool kKeysInLds = kRow == 256, kValuesInLds = kRow >= 256 && kRow <= 512;
+    static constexpr int kWaves = kRow == 128 ? 3 : kRow == 256 ? 2 : 1;                 // per SIMD
+    static constexpr bool kKeysInLds = kRow <= 256, kValuesInLds = kRow <= 512;
     static constexpr int kRows = kRow <= 128 ? 64 : 32;                                  // QT
     static constexpr size_t kLds = 2 * kRows * kRow + 2 * kRows * sizeof(float) + (kKeysInLds + kValuesInLds) * kKeys * kRow;
 };
@@ -250,9 +253,23 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
         if (lo < hi) { i_lo = (i32)(lo - r.start); i_hi = (i32)(hi - r.start); }
     }
     const Queries seen = queries_of(s, r.length, j);
-    const i32 first = i_lo / QT, per = i_lo < i_hi ? (i_hi + QT - 1) / QT - first : 0;
+    // Shares of the queries, whole tiles of QT.  With shares for lead tiles alone the first takes all the queries that see more
+    // than the leading keys, so that the others, and the partial sums, are about those keys only.
+    const bool apart = leads && a.splits == 1 && splits > 1;
+    i32 first = i_lo / QT, last = i_lo < i_hi ? (i_hi + QT - 1) / QT : first;
+    u32 parts = splits, part = split;
+    if (apart) {
+        i64 far = (i64)k1 + s.window - r.start;               // (positions from k1 + window on see no other key of the tile)
+        far = far < i_lo ? i_lo : far > i_hi ? i_hi : far;
+        i32 near = ((i32)far + QT - 1) / QT;
+        near = near < first ? first : near > last ? last : near;
+        if (split == 0) last = near; else first = near;
+        parts = split == 0 ? 1 : splits - 1;
+        part = split == 0 ? 0 : split - 1;
+    }
+    const i32 per = last - first;
     const u64 total = (u64)(u32)per * s.G;
-    const u64 from = total * split / splits, to = total * (split + 1) / splits;
+    const u64 from = total * part / parts, to = total * (part + 1) / parts;
 
     // the (head of the group, tile) of a step, stepped on by counting (a division per step costs more than its products)
     struct At { u32 g; i32 tile; };
@@ -325,7 +342,8 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
         }
     }
     if (j >= s.SK) return;
-    if (splits > 1) {
+    if (apart && split && j >= (i32)a.lead_keys) return;
+    if (splits > 1 && !(apart && j >= (i32)a.lead_keys)) {
         float *pk, *pv;
         share_of<DP>(a, split, head, (u32)j, &pk, &pv);
 #pragma unroll
@@ -402,17 +420,19 @@ template <class T, int DP> int backward(aixk_ctx* ctx, const Call& c, BackwardAr
     if (s.window && s.sinks && seen) {
         a.lead = ((u32)s.sinks + keys - 1) / keys;
         if (a.lead > a.tiles) a.lead = a.tiles;
-        a.lead_keys = a.lead * keys < (u32)s.SK ? a.lead * keys : (u32)s.SK;
     }
+    // keys with shares of their own: whole tiles if the other tiles have shares too, else the leading keys
+    auto lead_keys = [&](u64 sp) { return a.lead ? std::min<u64>(sp > 1 ? (u64)a.lead * keys : (u64)(u32)s.sinks, (u64)(u32)s.SK) : 0; };
     u64 splits = 1, planes = 0, grid = 0;
     double least = 0.0;
     for (u64 sp = 1; sp <= 64 && (sp == 1 || sp * 4 <= steps); ++sp) {
         const u64 n = heads * (a.lead * sp * more + (a.tiles - a.lead) * sp);
-        const u64 shares = (sp > 1 ? sp * rows : 0) + (sp * more > 1 ? (sp > 1 ? sp * (more - 1) : more) * heads * a.lead_keys : 0);
+        const u64 shares = (sp > 1 ? sp * rows : 0) + (sp * more > 1 ? (sp > 1 ? sp * (more - 1) : more) * heads * lead_keys(sp) : 0);
         const double cost = 2.0 * (double)((n + slots - 1) / slots) * (double)((steps + sp - 1) / sp + 3) + (shares ? 3.0 + (double)shares * (16.0 * DP / 4e6) : 0.0);
         if (sp == 1 || cost < least) { least = cost; splits = sp; planes = shares; grid = n; }
     }
     a.splits = (u32)splits;
+    a.lead_keys = (u32)lead_keys(splits);
     a.lead_splits = (u32)(a.lead ? splits * more : splits);
     AIXK_REQUIRE(grid < (1ull << 31), "attention_backward: too many rows");
     if (planes) {

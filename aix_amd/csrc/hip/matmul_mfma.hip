@@ -2275,7 +2275,8 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
             // few tiles and a long K (a weight gradient with ten output columns): K split over workgroups
             SplitArgs sk{};
             uint64_t ksplits = 1;
-            if (!only_if && n < (u32)ctx->cus && K >= 2048) ksplits = std::max<uint64_t>(1, std::min<uint64_t>({steps / 8, (fill + n - 1) / n, (uint64_t)64}));
+            // (for the operators of transformer blocks from 512 on: [11, 1792] x [1792, 64] F32_SHORT_US)
+            if (!only_if && n < (u32)ctx->cus && K >= (epi ? 512u : 2048u)) ksplits = std::max<uint64_t>(1, std::min<uint64_t>({steps / 8, (fill + n - 1) / n, (uint64_t)64}));
             sk.per_split = (u32)((steps + ksplits - 1) / ksplits);
             sk.splits = (u32)((steps + sk.per_split - 1) / sk.per_split);
             sk.matrices = 1;

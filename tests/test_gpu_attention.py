@@ -108,6 +108,14 @@ def test_windows_and_leading_keys(gpu, dtype, window, sinks, causal):
     both_ways(Case(gpu, dtype, 1, 2, 1, 300, 300, 64, causal=causal, window=window, sinks=sinks), f"window {window}, {sinks} leading keys")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal,window,sinks,heads,kv", [(True, 40, 4, 2, 2), (False, 40, 4, 2, 1), (True, 64, 140, 4, 2), (False, 30, 300, 2, 2), (True, 200, 129, 3, 1)])
+def test_leading_keys_far_from_their_queries(gpu, dtype, causal, window, sinks, heads, kv):
+    """Queries that see nothing but the leading keys have workgroups of their own in the backward pass."""
+    both_ways(Case(gpu, dtype, 2, heads, kv, 700, 700, 64, causal=causal, window=window, sinks=sinks, lengths=[700, 150]), f"window {window}, {sinks} leading keys")
+    both_ways(Case(gpu, dtype, 2, heads, kv, 650, 700, 64, causal=causal, window=window, sinks=sinks, lengths=[700, 3], starts=[20, 600]), f"window {window}, {sinks} leading keys, later")
+
+
 @pytest.mark.parametrize("dtype", [O.BF16, O.F16])
 @pytest.mark.parametrize("sq", [1, 3, 40, 150])
 @pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 20, 3), (False, 20, 3), (False, 0, 0)])
