@@ -614,26 +614,47 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
     const u64 rows = (u64)s.B * s.H * (u32)s.SQ;
     const u32 R = s.G * (u32)s.SQ;
     const u64 wide = (u64)s.B * s.H * (((u32)s.SQ + 127) / 128), narrow = (u64)s.B * s.HK * ((R + 15) / 16);
-    // Few queries: at most 32 rows per key head.
-    if (R > 32) {
-        if (sizeof(T) == 4 || wide < (u64)ctx->cus) {
-            const u64 grid = (u64)s.B * s.H * (((u32)s.SQ + 63) / 64);
-            AIXK_REQUIRE(grid < (1ull << 31), "attention: too many rows");
-            ForwardArgs a{s, c.q, c.k, c.v, c.out, c.lse, ((u32)s.SQ + 63) / 64, c.whole_out};
-            constexpr size_t lds = 2 * (DP * sizeof(T) <= 256 ? 64 : 32) * DP * sizeof(T);
-            AIXK_TRY(allow_lds(attention16_k<T, DP>, lds));
-            hipLaunchKernelGGL((attention16_k<T, DP>), dim3((unsigned)grid), dim3(256), lds, ctx->stream, a);
+    // Split or not, in steps of a workgroup on 64 keys (1.2 us at 128 dims in 16 bits).  Rows are worth a workgroup each 64 queries if
+    // its chain of steps is shorter than the rows' shares of the chip: a split step of 16 rows and 32 keys costs a wave 2.25 of
+    // them, several waves at a time in each SIMD, and joining shares costs 6.  bf16, 32 heads on 8, 128 dims, queries x keys:
+    // 128 x 8192 92 us split, 181 not; 40 x 32768 115 and 707; 8 heads of 512 x 512 20.9 and 15.8, 256 x 256 7.2 and 10.1.
+    // Up to 32 rows per key head, a single token among them, are split in any case.
+    constexpr int most = most_waves<T, DP>();
+    constexpr u64 resident = 163840 / SplitLds<T, DP, 4>::kBytes < 4 ? 163840 / SplitLds<T, DP, 4>::kBytes : 4;
+    // what a row can see at most: the whole cache, or the window and the leading keys
+    auto reach = [&](u64 span) {
+        const u64 inside = s.window ? (u64)s.window + span + (u64)s.sinks : (u64)s.SK;
+        return inside < (u64)s.SK ? inside : (u64)s.SK;
+    };
+    const u64 keys = reach(std::min<u64>((u64)(u32)s.SQ, 16));
+    const bool one = most > 4 && narrow < (u64)ctx->cus && keys > 4 * kSplitKeys && keys <= 3u * most * kSplitKeys;
+    const double block_steps = (double)((reach(64) + 63) / 64), split_steps = (double)((keys + kSplitKeys - 1) / kSplitKeys);
+    const double split_cost = one ? 2.25 * (double)(((u64)split_steps + most - 1) / most)
+                                  : 6.0 + 2.25 * (double)narrow * split_steps / (double)((u64)ctx->cus * 4 * std::min<u64>(resident, 2));
+    if (R > 32 && split_cost >= block_steps) {
+        // 32 queries to a wave where that leaves a workgroup for every compute unit, and above 128 head dims, where 16 queries to a
+        // wave read too much LDS for what they multiply (8 heads of 1000 x 192, few workgroups: 25.3 us against 36.0); f32 and
+        // small grids: 16 queries to a wave.
+        if constexpr (sizeof(T) == 4 || DP <= 128) {
+            if (sizeof(T) == 4 || wide < (u64)ctx->cus) {
+                const u64 grid = (u64)s.B * s.H * (((u32)s.SQ + 63) / 64);
+                AIXK_REQUIRE(grid < (1ull << 31), "attention: too many rows");
+                ForwardArgs a{s, c.q, c.k, c.v, c.out, c.lse, ((u32)s.SQ + 63) / 64, c.whole_out};
+                constexpr size_t lds = 2 * (DP * sizeof(T) <= 256 ? 64 : 32) * DP * sizeof(T);
+                AIXK_TRY(allow_lds(attention16_k<T, DP>, lds));
+                hipLaunchKernelGGL((attention16_k<T, DP>), dim3((unsigned)grid), dim3(256), lds, ctx->stream, a);
+                AIXK_HIP(hipGetLastError());
+                return AIXK_OK;
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+            AIXK_REQUIRE(wide < (1ull << 31), "attention: too many rows");
+            ForwardArgs a{s, c.q, c.k, c.v, c.out, c.lse, ((u32)s.SQ + 127) / 128, c.whole_out};
+            constexpr size_t lds = 2 * (DP <= 128 ? 64 : 32) * DP * sizeof(T);
+            AIXK_TRY(allow_lds(attention_k<T, DP>, lds));
+            hipLaunchKernelGGL((attention_k<T, DP>), dim3((unsigned)wide), dim3(256), lds, ctx->stream, a);
             AIXK_HIP(hipGetLastError());
             return AIXK_OK;
-        }
-        AIXK_REQUIRE(wide < (1ull << 31), "attention: too many rows");
-        if constexpr (sizeof(T) == 2) {
-        ForwardArgs a{s, c.q, c.k, c.v, c.out, c.lse, ((u32)s.SQ + 127) / 128, c.whole_out};
-        constexpr size_t lds = 2 * (DP <= 128 ? 64 : 32) * DP * sizeof(T);
-        AIXK_TRY(allow_lds(attention_k<T, DP>, lds));
-        hipLaunchKernelGGL((attention_k<T, DP>), dim3((unsigned)wide), dim3(256), lds, ctx->stream, a);
-        AIXK_HIP(hipGetLastError());
-        return AIXK_OK;
         }
     }
     SplitArgs a{s, c.q, c.k, c.v, c.out, c.lse, (R + 15) / 16, 1, c.whole_out, nullptr, nullptr};
@@ -646,18 +667,13 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
         return AIXK_OK;
     };
     AIXK_REQUIRE(narrow < (1ull << 31) && rows < (1ull << 31), "attention: too many rows");
-    // What a row can see at most bounds its steps: the whole cache, or the window and the leading keys.
-    u64 keys = (u64)s.SK;
-    if (s.window && (u64)s.window + (u64)s.SQ + (u64)s.sinks < keys) keys = (u64)s.window + (u64)s.SQ + (u64)s.sinks;
     // Few keys and few workgroups: one workgroup of as many waves as it holds takes them all in at most three steps, where
     // sharing them out costs a second launch (12 heads of 64 on 512 keys: 6.4 us with eight waves, 7.2 with sixteen, 4.8 + 3.4 in 4 shares).
-    constexpr int most = most_waves<T, DP>();
-    if (most > 4 && narrow < (u64)ctx->cus && keys > 4 * kSplitKeys && keys <= 3u * most * kSplitKeys) return launch(std::integral_constant<int, most>{});
+    if (one) return launch(std::integral_constant<int, most>{});
     // Otherwise shares of the keys until every compute unit has four workgroups, but no share below one step of all waves; up to
     // eight workgroups where a share still has eight steps (16 sequences of any length up to 32768: 193 us with shares for four
     // workgroups, 172 for eight, which even the lengths out; 2052 keys: 31.0 us with four, 34.2 with eight).
     const u64 steps = (keys + kSplitKeys * 4 - 1) / (kSplitKeys * 4);
-    constexpr u64 resident = 163840 / SplitLds<T, DP, 4>::kBytes < 4 ? 163840 / SplitLds<T, DP, 4>::kBytes : 4;
     u64 splits = ((u64)ctx->cus * resident + narrow - 1) / narrow;
     splits = std::max<u64>(splits, std::min<u64>(((u64)ctx->cus * 8 + narrow - 1) / narrow, steps / 8));
     if (splits > steps) splits = steps;

@@ -116,6 +116,25 @@ def test_leading_keys_far_from_their_queries(gpu, dtype, causal, window, sinks, 
     both_ways(Case(gpu, dtype, 2, heads, kv, 650, 700, 64, causal=causal, window=window, sinks=sinks, lengths=[700, 3], starts=[20, 600]), f"window {window}, {sinks} leading keys, later")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,heads,kv", [(5, 8, 4), (9, 16, 16)])
+@pytest.mark.parametrize("sq,sk,d", [(200, 200, 64), (130, 200, 40), (150, 150, 128), (129, 161, 192)])
+def test_many_rows(gpu, dtype, batch, heads, kv, sq, sk, d):
+    """Enough rows for workgroups of 64 queries, and of 128."""
+    lengths = [sk, 0, 1, sk - 1, sk // 2, 10 ** 6, -1, 65, 33][:batch]
+    for causal, window, sinks in ((True, 0, 0), (False, 0, 0), (True, 30, 3), (False, 70, 66)):
+        both_ways(Case(gpu, dtype, batch, heads, kv, sq, sk, d, causal=causal, window=window, sinks=sinks, lengths=lengths), f"causal {causal}, window {window}")
+    both_ways(Case(gpu, dtype, batch, heads, kv, sq, sk, d, window=50, sinks=2, lengths=lengths, starts=[5, 0, -3, 70, 2 ** 31 - 1, -2 ** 31, sk - 1, 0, 40][:batch]), "starts")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv,sq,d", [(8, 2, 64, 64), (4, 4, 50, 128), (6, 2, 33, 80), (2, 2, 100, 192), (4, 1, 17, 256)])
+def test_some_queries_far_into_a_cache(gpu, dtype, heads, kv, sq, d):
+    """The next part of a prompt: the keys of its rows in shares."""
+    for window, sinks in ((0, 0), (300, 4)):
+        both_ways(Case(gpu, dtype, 2, heads, kv, sq, 3000, d, window=window, sinks=sinks, lengths=[3000, 1234]), f"{sq} queries, window {window}")
+
+
 @pytest.mark.parametrize("dtype", [O.BF16, O.F16])
 @pytest.mark.parametrize("sq", [1, 3, 40, 150])
 @pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 20, 3), (False, 20, 3), (False, 0, 0)])
