@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_k(Fo
 
 // The same on 16 queries per wave, 64 per workgroup, with v_mfma 16x16: for f32, whose matrix instructions are a sixteenth as
 // fast (a wave of 32 queries takes 7 us for a tile of 64 keys: half the queries are twice the waves to fill the chip with, and
-// the head dim's tail is left out), and for grids of 128-query workgroups that leave compute units without one.
+// the head dim's tail is left out), and up to 128 head dims for grids of 128-query workgroups that leave compute units without one.
 template <class T, int DP>
 __global__ __launch_bounds__(256, DP * sizeof(T) <= 512 ? 2 : 1) void attention16_k(ForwardArgs a)
 {
@@ -589,7 +589,7 @@ int pack(aixk_ctx* ctx, int dtype, const View& src, void* dst, u32 B, u32 H, u64
 {
     const u64 rows = (u64)B * H * S;
     if (!rows || !DW) return AIXK_OK;
-    AIXK_REQUIRE(S < (1ull << 32) && (u64)B * H < (1ull << 32), "operand copy: shape too large");
+    AIXK_REQUIRE(S < (1ull << 31) && (u64)B * H < (1ull << 32), "operand copy: shape too large");
     const u32 words = DW / (16 / (u32)aixk_dtype_size(dtype));
     u32 lanes = 1;
     while (lanes < words && lanes < 64) lanes *= 2;
@@ -612,7 +612,7 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
 {
     const Shape& s = c.s;
     const u64 rows = (u64)s.B * s.H * (u32)s.SQ;
-    const u32 R = s.G * (u32)s.SQ;
+    const u64 R = (u64)s.G * (u32)s.SQ;
     const u64 wide = (u64)s.B * s.H * (((u32)s.SQ + 127) / 128), narrow = (u64)s.B * s.HK * ((R + 15) / 16);
     // Split or not, in steps of a workgroup on 64 keys (1.2 us at 128 dims in 16 bits).  Rows are worth a workgroup each 64 queries if
     // its chain of steps is shorter than the rows' shares of the chip: a split step of 16 rows and 32 keys costs a wave 2.25 of
@@ -631,7 +631,7 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
     const double block_steps = (double)((reach(64) + 63) / 64), split_steps = (double)((keys + kSplitKeys - 1) / kSplitKeys);
     const double split_cost = one ? 2.25 * (double)(((u64)split_steps + most - 1) / most)
                                   : 6.0 + 2.25 * (double)narrow * split_steps / (double)((u64)ctx->cus * 4 * std::min<u64>(resident, 2));
-    if (R > 32 && split_cost >= block_steps) {
+    if (R > 32 && (split_cost >= block_steps || R >= (1ull << 31))) {
         // 32 queries to a wave where that leaves a workgroup for every compute unit, and above 128 head dims, where 16 queries to a
         // wave read too much LDS for what they multiply (8 heads of 1000 x 192, few workgroups: 25.3 us against 36.0); f32 and
         // small grids: 16 queries to a wave.
@@ -657,7 +657,7 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
             return AIXK_OK;
         }
     }
-    SplitArgs a{s, c.q, c.k, c.v, c.out, c.lse, (R + 15) / 16, 1, c.whole_out, nullptr, nullptr};
+    SplitArgs a{s, c.q, c.k, c.v, c.out, c.lse, (u32)((R + 15) / 16), 1, c.whole_out, nullptr, nullptr};
     auto launch = [&](auto waves_tag) -> int {
         constexpr int WAVES = decltype(waves_tag)::value;
         constexpr size_t lds = SplitLds<T, DP, WAVES>::kBytes;
@@ -670,8 +670,8 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
     // Few keys and few workgroups: one workgroup of as many waves as it holds takes them all in at most three steps, where
     // sharing them out costs a second launch (12 heads of 64 on 512 keys: 6.4 us with eight waves, 7.2 with sixteen, 4.8 + 3.4 in 4 shares).
     if (one) return launch(std::integral_constant<int, most>{});
-    // Otherwise shares of the keys until every compute unit has four workgroups, but no share below one step of all waves; up to
-    // eight workgroups where a share still has eight steps (16 sequences of any length up to 32768: 193 us with shares for four
+    // Otherwise shares of the keys until every compute unit has the workgroups its LDS holds, four at most (f32 at 256 dims holds one:
+    // 4 x 8 heads on 4 of 8192 keys 72 us), but no share below one step of all waves; up to eight workgroups where a share still has eight steps (16 sequences of any length up to 32768: 193 us with shares for four
     // workgroups, 172 for eight, which even the lengths out; 2052 keys: 31.0 us with four, 34.2 with eight).
     const u64 steps = (keys + kSplitKeys * 4 - 1) / (kSplitKeys * 4);
     u64 splits = ((u64)ctx->cus * resident + narrow - 1) / narrow;

@@ -412,7 +412,7 @@ template <class T, int DP> int backward(aixk_ctx* ctx, const Call& c, BackwardAr
     // Shares of the queries by a cost in microseconds: rounds of workgroups, each of its steps (about 2 us, three of them the
     // workgroup's own), and the shares written and read again (4 TB/s, and the joining launch).  Key tiles with leading keys, which
     // every query sees, take as many more shares as they have more queries.  16 heads on 4 of 4096 x 128, window 1024: 3 shares
-    // SHARE3_US, 8 shares 148 us.
+    // 98 us and 13 for joining them, 8 shares 148 in all.
     constexpr u64 resident = KeyBlock<T, DP>::kWaves * 256 / KeyBlock<T, DP>::kThreads;
     const u64 slots = (u64)ctx->cus * resident;
     const u64 seen = s.window && (u64)s.window + keys < (u64)(u32)s.SQ ? (u64)s.window + keys : (u64)(u32)s.SQ;      // queries of a tile at most

@@ -1603,7 +1603,11 @@ int workspace(aixk_ctx* ctx, int which, size_t bytes, void** out)
 
 template <class K> int set_lds(K kernel, size_t bytes)
 {
-    static std::unordered_map<const void*, size_t> done;          // kernel -> dynamic LDS limit already raised
+    static thread_local std::unordered_map<const void*, size_t> done;     // kernel -> dynamic LDS limit already raised, on `device`
+    static thread_local int device = -1;
+    int now = 0;
+    AIXK_HIP(hipGetDevice(&now));
+    if (now != device) { done.clear(); device = now; }
     auto it = done.find((const void*)kernel);
     if (it == done.end() || it->second < bytes) {
         AIXK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
@@ -2275,7 +2279,7 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
             // few tiles and a long K (a weight gradient with ten output columns): K split over workgroups
             SplitArgs sk{};
             uint64_t ksplits = 1;
-            // (for the operators of transformer blocks from 512 on: [11, 1792] x [1792, 64] F32_SHORT_US)
+            // (for the operators of transformer blocks from 512 on: [11, 1792] x [1792, 64] 45 -> 14.5 us)
             if (!only_if && n < (u32)ctx->cus && K >= (epi ? 512u : 2048u)) ksplits = std::max<uint64_t>(1, std::min<uint64_t>({steps / 8, (fill + n - 1) / n, (uint64_t)64}));
             sk.per_split = (u32)((steps + ksplits - 1) / ksplits);
             sk.splits = (u32)((steps + sk.per_split - 1) / sk.per_split);
@@ -2360,7 +2364,7 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
 // A product that nothing follows, for the operators of transformer blocks: aixk_matmul's own kernels where they take the shape.
 // What would be left to its LDS-tiled kernel -- contractions without whole 16-byte words (the rows of a batch in a weight
 // gradient), results below 64 x 64 elements -- has its operands copied K-contiguous with zeros up to a whole word.
-// (f32 [1216, 11127] x [11127, 128] XODD_US; f32 [1, 2624] x [2624, 64] XTINY_US.)
+// (f32, the backward pass of [11127, 1216] x [1216, 128]: 2334 -> 130 us; [1, 2624] x [2624, 64]: 347 -> 15 us.)
 int matmul_plain(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out)
 {
     const uint64_t M = a->shape[0], K = a->shape[1], N = b->shape[1];

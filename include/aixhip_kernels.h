@@ -240,7 +240,9 @@ int32_t aixk_matmul_grouped(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_
  * lengths NULL: every key; starts NULL: the queries are the last ones, starts[b] = lengths[b] - queries.  Both are int32
  * [batch] in device memory, read when the kernels run (a captured call follows their current values); lengths beyond the
  * keys count as all of them, negative ones as none; starts are taken within +- 2^29.  Keys at and behind a length are never
- * read.  A query that sees no key gives zeros and lse = -infinity, and no gradient. */
+ * read.  A query that sees no key gives zeros and lse = -infinity, and no gradient.  Unseen pairs in
+ * front of a length take part in the products with a weight of zero: keys and values there, queries and their gradients must be
+ * finite (their scores need not be). */
 typedef struct aixk_attention_spec {
     float    scale;                  /* factor of the scores, positive and finite */
     int32_t  causal;
