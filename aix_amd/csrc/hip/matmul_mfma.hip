@@ -2233,14 +2233,17 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
         // long K, K is split over workgroups
         // two workgroups per compute unit hide each other's split-and-stage phases: with fewer tiles than that, K is split
         // over workgroups if it is long enough, else the f32 MFMA kernels below take the product
+        // (the operators of transformer blocks split further where the tiles are whole: [1974, 5888] x [5888, 384] 121 -> 78 us,
+        // [3410, 3328] x [3328, 256] 76 -> 55, but 64 rows, half a tile, on [4096, 4096] 39 us against 33)
+        const bool tall = epi && M >= 128 && N >= 128;
         uint64_t splits = 1;
         // (as many splits as still fit one round of two workgroups per compute unit: [784, 4096]^T x [4096, 2048], 112 tiles,
         // takes 107 us with 4 splits and 131 with 5, whose 560 workgroups spill into a second round)
         if (t128 < fill && K >= 2048) {
             const uint64_t whole = fill / t128, over = (fill + t128 - 1) / t128;
-            splits = std::max<uint64_t>(1, std::min<uint64_t>({steps / 16, t128 * whole >= fill - fill / 8 ? whole : over, (uint64_t)64}));
+            splits = std::max<uint64_t>(1, std::min<uint64_t>({steps / (tall ? 8 : 16), t128 * whole >= fill - fill / 8 ? whole : over, (uint64_t)64}));
         }
-        if (!only_if && t128 * splits >= fill - fill / 8 && t128 >= (uint64_t)ctx->cus / 4) {
+        if (!only_if && t128 * splits >= fill - fill / 8 && t128 >= (uint64_t)ctx->cus / (tall ? 8 : 4)) {
             const u32 n = grid_of(g, 128, 128);
             SplitArgs sk{};
             sk.per_split = (u32)((steps + splits - 1) / splits);
@@ -2279,7 +2282,7 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
             // few tiles and a long K (a weight gradient with ten output columns): K split over workgroups
             SplitArgs sk{};
             uint64_t ksplits = 1;
-            // (for the operators of transformer blocks from 512 on: [11, 1792] x [1792, 64] 45 -> 14.5 us)
+            // (for the operators of transformer blocks from 512 on: [11, 1792] x [1792, 64] 45 -> 14.5 us, [300, 1000] x [1000, 300] 31 -> 15)
             if (!only_if && n < (u32)ctx->cus && K >= (epi ? 512u : 2048u)) ksplits = std::max<uint64_t>(1, std::min<uint64_t>({steps / 8, (fill + n - 1) / n, (uint64_t)64}));
             sk.per_split = (u32)((steps + ksplits - 1) / ksplits);
             sk.splits = (u32)((steps + sk.per_split - 1) / sk.per_split);
@@ -2361,7 +2364,7 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
     return AIXK_OK;
 }
 
-// A product that nothing follows, for the operators of transformer blocks: aixk_matmul's own kernels where they take the shape.
+// A product that nothing follows, for the operators of transformer blocks: aixk_matmul's own kernels, with their K split further.
 // What would be left to its LDS-tiled kernel -- contractions without whole 16-byte words (the rows of a batch in a weight
 // gradient), results below 64 x 64 elements -- has its operands copied K-contiguous with zeros up to a whole word.
 // (f32, the backward pass of [11127, 1216] x [1216, 128]: 2334 -> 130 us; [1, 2624] x [2624, 64]: 347 -> 15 us.)
@@ -2370,7 +2373,7 @@ int matmul_plain(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, 
     const uint64_t M = a->shape[0], K = a->shape[1], N = b->shape[1];
     const size_t esz = aixk_dtype_size(out->dtype);
     const uint64_t word = 16 / esz, Kp = (K + word - 1) / word * word;
-    if (K == 0 || (K == Kp && M * N >= 64 * 64)) return aixk_matmul(ctx, a, b, out);
+    if (K == 0 || (esz == 2 && K == Kp && M * N >= 64 * 64)) return aixk_matmul(ctx, a, b, out);
     EpiArgs nothing{};
     nothing.whole = N % 8 == 0 && aligned16(out->data);
     if (esz == 2) return matmul_mfma_epilogue(ctx, a, b, out, nothing);
