@@ -165,6 +165,13 @@ def test_backward_parts(gpu, dtype, act):
     backward(gpu, dtype, 3000, 8, 24, act)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [1, 2, 7, 9, 31, 33, 65, 127, 1001, 4099])
+@pytest.mark.parametrize("k,n", [(64, 64), (8, 16), (136, 264), (7, 24), (200, 65)])
+def test_weight_gradients_of_any_number_of_rows(gpu, dtype, m, k, n):
+    backward(gpu, dtype, m, k, n)
+
+
 def test_gradients_against_differences(gpu):
     """f32: the directional derivative of sum(out w), by a central difference of the kernel's own forward pass with step 2^-7;
     the third derivative (step^2) and the rounding of the two sums stay below 2 % of the gradient's length."""
