@@ -135,14 +135,6 @@ __device__ __forceinline__ Tiles tiles_of(const Shape& s, i32 length, i32 p0, i3
 }
 __device__ __forceinline__ i32 tile_at(const Tiles& t, i32 i) { return i < t.sink ? i : t.first + i - t.sink; }
 
-// Workgroups go round the 8 XCDs one by one; number them so that each XCD works on a contiguous run (the tiles of one key
-// head share its keys in that XCD's L2).  A bijection for any n.
-__device__ __forceinline__ u32 xcd_order(u32 id, u32 n)
-{
-    const u32 q = n / 8u, r = n % 8u, x = id % 8u;
-    return x * q + (x < r ? x : r) + id / 8u;
-}
-
 // A grid of `heads` x ranks: workgroup id stands for the (id / heads)-th rank -- the heaviest first -- of head id % heads.  Ids go
 // round the XCDs, so with a multiple of eight key heads a key head and all query heads on it stay on one XCD, whose L2 then
 // holds its keys, and every XCD gets every rank.  Sequences of different lengths are moved on by one from rank to rank: the long

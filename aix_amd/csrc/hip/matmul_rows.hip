@@ -29,6 +29,13 @@ struct RowsArgs {
 
 constexpr int kWaves = 8, kAhead = 4;
 
+// Workgroups go round the 8 XCDs one by one; number them so that each XCD works on a contiguous run of columns.  A bijection for any n.
+__device__ __forceinline__ u32 xcd_order(u32 id, u32 n)
+{
+    const u32 q = n / 8u, r = n % 8u, x = id % 8u;
+    return x * q + (x < r ? x : r) + id / 8u;
+}
+
 // slot of 16-byte word c of K row k in a slab: the transposed reads take 32 bytes from each of eight K rows at a time
 template <int WORDS> __device__ __forceinline__ int turn(int k)
 {
