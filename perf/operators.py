@@ -4,7 +4,11 @@ product with bias, activation and residual in its epilogue (forward and backward
 
 A case is a dict of plain values; prepare() makes its tensors, run() is one call -- in elementary torch operations
 where `own` is false, through the kernel layer (aix_amd.kernels, include/aixhip_kernels.h) where it is true -- and
-exact() is the operator's definition in 64 bits."""
+exact() is the operator's definition in 64 bits.
+
+The kernel layer's calls run on a stream of their context, which does not wait for torch's nor torch's for it: prepare() ends
+with its inputs complete, and a program waits for the device (torch.cuda.synchronize()) before it reads the results of
+run() or drops a state that a run() still uses."""
 import ctypes
 import math
 
@@ -161,6 +165,7 @@ def prepare(case, seed):
                          "db": torch.empty((k, n), dtype=dt, device="cuda"), "dbias": torch.empty((n,), dtype=dt, device="cuda")}
     if own:
         s["call"] = _bind(s)    # the framework's tensors are descriptors; a program that holds the tensors holds these
+        torch.cuda.synchronize()
     return s
 
 
