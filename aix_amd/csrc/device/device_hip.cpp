@@ -786,11 +786,26 @@ void DeviceHIP::requireDevice(const DeviceTensorParams& result, const char* op) 
 
 const void* DeviceHIP::stageRaw(const void* src, size_t bytes)
 {
+    const Staging hold_(this);
     void* tmp = allocateBlock(bytes, false);
+    try { m_staged.emplace_back(tmp, bucketBytes(bytes)); }
+    catch (...) { aixk_free(m_ctx, tmp, 0); throw; }
     check(aixk_copy_in(m_ctx, tmp, src, bytes));
-    m_limbo.emplace_back(tmp, bucketBytes(bytes));          // recycled after the work that reads it is enqueued
-    m_limboBytes += bucketBytes(bytes);
     return tmp;
+}
+
+// Staged blocks are recycled after the work that reads them is enqueued.  (Runs in destructors: without host memory for the
+// list the blocks are given up.)
+void DeviceHIP::endStaging()
+{
+    try {
+        for (const auto& b : m_staged) {
+            m_limbo.push_back(b);
+            m_limboBytes += b.second;
+        }
+    } catch (...) {
+    }
+    m_staged.clear();
 }
 
 void DeviceHIP::onDevice(View& v)
@@ -835,6 +850,7 @@ void DeviceHIP::stagedPod(const DeviceTensorParams& p, aixhip_tensor* out, const
 void DeviceHIP::recordBinary(OpType t, const DeviceTensorParams& a, const DeviceTensorParams& b, const DeviceTensorParams& r, const char* op)
 {
     const Marker marker_(op);
+    const Staging hold_(this);
     requireDevice(r, op);
     if (a.dtype != r.dtype || b.dtype != r.dtype)
         throw std::invalid_argument(std::string("DeviceHIP::") + op + "() operands must have the result's data type.");
@@ -1362,6 +1378,7 @@ void DeviceHIP::matmul(const DeviceTensorParams& a, const DeviceTensorParams& b,
             return;
         }
     }
+    const Staging hold_(this);
     flushFor(a.data, b.data, result.data);
     aixhip_tensor pa, pb, pr; stagedPod(a, &pa, "matmul"); stagedPod(b, &pb, "matmul"); toPod(result, &pr, "matmul");
     // operands with leading dims in front of the matrix dims: a stack of products (beyond the reference, whose
@@ -1808,6 +1825,7 @@ void DeviceHIP::indexSelect(const DeviceTensorParams& src, const DeviceTensorPar
 {
     const Marker marker_("indexSelect");
     AIXHIP_TRACE("indexSelect");
+    const Staging hold_(this);
     requireDevice(dst, "indexSelect");
     flushFor(src.data, indices.data, dst.data);
     aixhip_tensor ps, pd, pi; stagedPod(src, &ps, "indexSelect"); toPod(dst, &pd, "indexSelect"); stagedPod(indices, &pi, "indexSelect");
@@ -1818,6 +1836,7 @@ void DeviceHIP::indexAdd(const DeviceTensorParams& src, const DeviceTensorParams
 {
     const Marker marker_("indexAdd");
     AIXHIP_TRACE("indexAdd");
+    const Staging hold_(this);
     requireDevice(dst, "indexAdd");
     flushFor(src.data, indices.data, dst.data);
     aixhip_tensor ps, pd, pi; stagedPod(src, &ps, "indexAdd"); toPod(dst, &pd, "indexAdd"); stagedPod(indices, &pi, "indexAdd");
@@ -1829,11 +1848,12 @@ void DeviceHIP::indexAdd(const DeviceTensorParams& src, const DeviceTensorParams
 struct DeviceHIP::BlockCall {
     DeviceHIP* dev;
     const char* op;
+    Staging hold;
     std::array<aixhip_tensor, 16> pods{};
     std::array<const void*, 16> named{};
     std::array<bool, 16> writes{};
     size_t count{0};
-    BlockCall(DeviceHIP* d, const char* name) : dev(d), op(name) {}
+    BlockCall(DeviceHIP* d, const char* name) : dev(d), op(name), hold(d) {}
     // a result must be this device's memory; an operand in host memory is staged by ready()
     void note(const DeviceTensorParams* p, bool write)
     {

@@ -188,6 +188,16 @@ private:
     // Makes the view's data device memory: a host operand is staged into a temporary block.
     void onDevice(aixhip::fuse::View& v);
     const void* stageRaw(const void* src, size_t bytes);
+    // While one lives, staged blocks are held for the operator under way: running out of memory -- for its next operand, or in
+    // the kernel layer -- gives idle blocks back to the driver, and these are not idle.  Then they go the way of freed blocks.
+    struct Staging {
+        DeviceHIP* dev;
+        explicit Staging(DeviceHIP* d) : dev(d) { ++dev->m_stagings; }
+        ~Staging() { if (--dev->m_stagings == 0) dev->endStaging(); }
+        Staging(const Staging&) = delete;
+        Staging& operator=(const Staging&) = delete;
+    };
+    void endStaging();
     void toPod(const DeviceTensorParams& p, aixhip_tensor* out, const char* op) const;
     void toPod(const aixhip::fuse::View& v, aixhip_tensor* out) const;
     void stagedPod(const DeviceTensorParams& p, aixhip_tensor* out, const char* op);      // toPod + staging of a host operand
@@ -217,6 +227,8 @@ private:
     BlockTable m_blocks;
     std::unordered_map<size_t, std::vector<void*>> m_pool;     // free blocks by bucket size
     std::vector<std::pair<void*, size_t>> m_limbo;             // freed, but recorded work may still use them
+    std::vector<std::pair<void*, size_t>> m_staged;            // copies of host operands of the operator under way (Staging)
+    int m_stagings{0};
     size_t m_liveBytes{0}, m_pooledBytes{0}, m_limboBytes{0}, m_totalBytes{0}, m_cacheLimit{~size_t(0)};
     void trimPool();
     void pool(void* p, size_t bytes);     // an idle block goes back to its bucket, or aside if a graph uses it

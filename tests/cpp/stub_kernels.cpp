@@ -11,6 +11,8 @@
 #include <cstdlib>
 #include <cstring>
 #include <deque>
+#include <initializer_list>
+#include <map>
 #include <string>
 
 struct aixk_module { std::string entry; };
@@ -18,12 +20,31 @@ struct aixk_ctx {
     size_t budget{SIZE_MAX}, held{0}; int event_delay{0}; uint64_t launches{0}, allocs{0}, frees{0}, syncs{0}, hits{0}, misses{0};
     std::string log;                                       // what was launched, in order: "name;name;..." (generated kernels by their entry)
     std::deque<aixk_module> modules;
+    std::map<const char*, size_t> live;                    // blocks handed out and not returned
+    uint64_t dead_operands{0};                             // data pointers that compute calls were given outside of any of them
 };
 struct aixk_event { int countdown{0}; bool recorded{false}; };
 
 static thread_local char g_error[256] = "";
 static std::atomic<long long> g_held_everywhere{0};        // bytes handed out and not yet returned, over all contexts
 static std::atomic<int> g_fail_matmuls{0};                 // the next n matmul calls report AIXK_ENOMEM
+static std::atomic<int> g_fail_blocks{0};                  // the same for the operators of transformer blocks
+// the operands of a call that enqueues work on them
+static void look(aixk_ctx* c, std::initializer_list<const aixhip_tensor*> operands)
+{
+    for (const aixhip_tensor* t : operands) {
+        if (!t || !t->data || t->size == 0) continue;
+        auto it = c->live.upper_bound((const char*)t->data);
+        if (it == c->live.begin() || (const char*)t->data >= (--it)->first + it->second) ++c->dead_operands;
+    }
+}
+static int32_t block_call(aixk_ctx* c, const char* name, std::initializer_list<const aixhip_tensor*> operands)
+{
+    look(c, operands);
+    if (g_fail_blocks > 0) { --g_fail_blocks; std::snprintf(g_error, sizeof(g_error), "stub: workspace of %s", name); return AIXK_ENOMEM; }
+    ++c->launches; c->log += std::string(name) + ";";
+    return AIXK_OK;
+}
 
 extern "C" {
 
@@ -37,6 +58,8 @@ uint64_t stub_frees(aixk_ctx* c) { return c->frees; }
 uint64_t stub_syncs(aixk_ctx* c) { return c->syncs; }
 long long stub_held_everywhere(void) { return g_held_everywhere.load(); }
 void stub_fail_next_matmuls(int n) { g_fail_matmuls = n; }
+void stub_fail_next_blocks(int n) { g_fail_blocks = n; }
+uint64_t stub_dead_operands(aixk_ctx* c) { return c->dead_operands; }
 const char* stub_log(aixk_ctx* c) { return c->log.c_str(); }
 void stub_log_clear(aixk_ctx* c) { c->log.clear(); }
 
@@ -59,12 +82,14 @@ int32_t aixk_alloc(aixk_ctx* c, size_t bytes, int, void** out)
     *(size_t*)p = bytes;                                   // size header in front of the 256-byte aligned block
     c->held += bytes; ++c->allocs; g_held_everywhere += (long long)bytes;
     *out = (char*)p + 256;
+    c->live[(const char*)*out] = bytes;
     return AIXK_OK;
 }
 int32_t aixk_free(aixk_ctx* c, void* ptr, int)
 {
     if (!ptr) return AIXK_OK;
     void* base = (char*)ptr - 256;
+    c->live.erase((const char*)ptr);
     c->held -= *(size_t*)base; ++c->frees; g_held_everywhere -= (long long)*(size_t*)base;
     std::free(base);
     return AIXK_OK;
@@ -76,7 +101,12 @@ int32_t aixk_zero(aixk_ctx* c, void* d, size_t n) { ++c->launches; std::memset(d
 int32_t aixk_sync(aixk_ctx* c) { ++c->syncs; return AIXK_OK; }
 
 #define STUB_OP(name, ...) int32_t name(aixk_ctx* c, __VA_ARGS__) { ++c->launches; c->log += #name ";"; return AIXK_OK; }
-STUB_OP(aixk_binary, int, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*)
+int32_t aixk_binary(aixk_ctx* c, int, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* r)
+{
+    look(c, {a, b, r});
+    ++c->launches; c->log += "aixk_binary;";
+    return AIXK_OK;
+}
 STUB_OP(aixk_unary, int, const aixhip_tensor*, const aixhip_tensor*)
 STUB_OP(aixk_fill, const void*, int, const aixhip_tensor*)
 STUB_OP(aixk_fill_min, const aixhip_tensor*)
@@ -87,8 +117,18 @@ STUB_OP(aixk_slice_set, const aixhip_tensor*, const aixhip_tensor*, uint64_t, ui
 STUB_OP(aixk_slice_set_many, const aixk_slice_item*, uint32_t)
 STUB_OP(aixk_slice_set_init, const aixhip_tensor*, const aixhip_tensor*, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t)
 STUB_OP(aixk_tri, int, const aixhip_tensor*, const aixhip_tensor*, int64_t)
-STUB_OP(aixk_index_select, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, uint64_t)
-STUB_OP(aixk_index_add, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, uint64_t)
+int32_t aixk_index_select(aixk_ctx* c, const aixhip_tensor* a, const aixhip_tensor* r, const aixhip_tensor* i, uint64_t)
+{
+    look(c, {a, r, i});
+    ++c->launches; c->log += "aixk_index_select;";
+    return AIXK_OK;
+}
+int32_t aixk_index_add(aixk_ctx* c, const aixhip_tensor* a, const aixhip_tensor* r, const aixhip_tensor* i, uint64_t)
+{
+    look(c, {a, r, i});
+    ++c->launches; c->log += "aixk_index_add;";
+    return AIXK_OK;
+}
 STUB_OP(aixk_reduce_all, int, const aixhip_tensor*, const aixhip_tensor*)
 STUB_OP(aixk_reduce_all_noalloc, int, const aixhip_tensor*, const aixhip_tensor*)
 STUB_OP(aixk_reduce_to, int, const aixhip_tensor*, const aixhip_tensor*)
@@ -98,19 +138,24 @@ STUB_OP(aixk_argmax_onehot_many, const aixk_argmax_item*, uint32_t)
 STUB_OP(aixk_sum_columns_many, const aixk_colsum_item*, uint32_t)
 STUB_OP(aixk_sum_partials, const void*, uint64_t, const aixhip_tensor*, uint64_t)
 STUB_OP(aixk_sum_partials_many, const aixk_partials_item*, uint32_t)
-int32_t aixk_matmul(aixk_ctx* c, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*)
+int32_t aixk_matmul(aixk_ctx* c, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* r)
 {
+    look(c, {a, b, r});
     if (g_fail_matmuls > 0) { --g_fail_matmuls; std::snprintf(g_error, sizeof(g_error), "stub: matmul workspace"); return AIXK_ENOMEM; }
     ++c->launches; c->log += "aixk_matmul;";
     return AIXK_OK;
 }
-STUB_OP(aixk_attention, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixk_attention_spec*, const aixhip_tensor*, const aixhip_tensor*)
-STUB_OP(aixk_attention_backward, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*,
-        const aixk_attention_spec*, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*)
-STUB_OP(aixk_rotary, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixk_rotary_spec*, const aixhip_tensor*, const aixhip_tensor*)
-STUB_OP(aixk_matmul_epilogue, const aixhip_tensor*, const aixhip_tensor*, const aixk_epilogue*, const aixhip_tensor*)
-STUB_OP(aixk_matmul_epilogue_backward, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*, int32_t, const aixhip_tensor*,
-        const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*)
+typedef const aixhip_tensor* T;
+int32_t aixk_attention(aixk_ctx* c, T q, T k, T v, const aixk_attention_spec* s, T out, T lse)
+{ return block_call(c, "aixk_attention", {q, k, v, s->lengths, s->starts, out, lse}); }
+int32_t aixk_attention_backward(aixk_ctx* c, T grad, T q, T k, T v, T out, T lse, const aixk_attention_spec* s, T dq, T dk, T dv)
+{ return block_call(c, "aixk_attention_backward", {grad, q, k, v, out, lse, s->lengths, s->starts, dq, dk, dv}); }
+int32_t aixk_rotary(aixk_ctx* c, T q, T k, T positions, const aixk_rotary_spec*, T q_out, T k_out)
+{ return block_call(c, "aixk_rotary", {q, k, positions, q_out, k_out}); }
+int32_t aixk_matmul_epilogue(aixk_ctx* c, T a, T b, const aixk_epilogue* e, T out)
+{ return block_call(c, "aixk_matmul_epilogue", {a, b, e->bias, e->residual, e->pre, out}); }
+int32_t aixk_matmul_epilogue_backward(aixk_ctx* c, T grad, T a, T b, T pre, int32_t, T dz, T da, T db, T dbias)
+{ return block_call(c, "aixk_matmul_epilogue_backward", {grad, a, b, pre, dz, da, db, dbias}); }
 STUB_OP(aixk_matmul_batched, const aixhip_tensor*, const aixhip_tensor*, const aixhip_tensor*)
 int32_t aixk_matmul_grouped(aixk_ctx* c, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out, uint32_t count)
 {

@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstdlib>
+#include <functional>
 #include <random>
 #include <set>
 #include <stdexcept>
@@ -26,6 +27,8 @@ uint64_t stub_frees(aixk_ctx*);
 uint64_t stub_syncs(aixk_ctx*);
 long long stub_held_everywhere(void);
 void stub_fail_next_matmuls(int);
+void stub_fail_next_blocks(int);
+uint64_t stub_dead_operands(aixk_ctx*);
 const char* stub_log(aixk_ctx*);
 void stub_log_clear(aixk_ctx*);
 }
@@ -541,6 +544,67 @@ static void test_blocks_of_a_captured_step_stay_with_the_graph()
     CHECK(dev.allocatedBytes() == 0);
 }
 
+// Operands in host memory are copied into blocks of the device's own.  Running out of memory on the way -- the kernel layer's
+// workspace, or the block of the next operand -- gives idle blocks back to the driver: not those.
+static void test_copies_of_host_operands_outlive_an_out_of_memory_retry()
+{
+    DeviceHIP dev;
+    aixk_ctx* ctx = dev.kernelContext();
+    std::vector<float> host(1 << 18, 1.5f);
+    std::vector<int32_t> ints(64, 0);
+    float* r = (float*)dev.allocate(sizeof(float) << 18);
+    auto at = [&](void* p, std::vector<size_t> shape) { return tensor(p, std::move(shape)); };
+    const auto h4 = at(host.data(), {2, 2, 4, 8}), r4 = at(r, {2, 2, 4, 8}), lse = at(r + 256, {2, 2, 4}), h2 = at(host.data(), {8, 8}), r2 = at(r, {8, 8}), s2 = at(r + 256, {8, 8});
+    const auto lengths = tensor(ints.data(), {2}, DataType::kInt32), positions = tensor(ints.data(), {2, 4}, DataType::kInt32);
+    aix::hip::AttentionSpec spec;
+    spec.lengths = &lengths;
+    aix::hip::RotarySpec turn;
+    turn.dims = 8;
+    aix::hip::Epilogue epilogue;
+    epilogue.bias = &h2; epilogue.residual = &h2;
+    const std::vector<std::function<void()>> calls = {
+        [&] { dev.attention(h4, h4, h4, spec, r4, &lse); },
+        [&] { dev.attentionBackward(h4, h4, h4, h4, h4, at(host.data(), {2, 2, 4}), spec, r4, at(r + 512, {2, 2, 4, 8}), at(r + 1024, {2, 2, 4, 8})); },
+        [&] { dev.rotary(h4, &h4, positions, turn, r4, &s2); },
+        [&] { dev.matmulEpilogue(h2, h2, epilogue, r2); },
+        [&] { dev.matmulEpilogueBackward(h2, h2, h2, &h2, aix::hip::Activation::kGELU, &r2, &s2, nullptr, nullptr); },
+        [&] { dev.matmul(h2, h2, r2); },
+    };
+    for (const auto& call : calls) {
+        stub_fail_next_blocks(1); stub_fail_next_matmuls(1);
+        call();
+        CHECK(stub_dead_operands(ctx) == 0);
+    }
+    stub_fail_next_blocks(0); stub_fail_next_matmuls(0);
+    // the second operand's block is what no room is left for
+    const std::vector<std::function<void()>> pairs = {
+        [&] { dev.matmul(at(host.data(), {4, 4}), at(host.data(), {4, 40000}), at(r, {4, 40000})); },
+        [&] { dev.add(at(host.data(), {1, 1, 1, 1, 1, 1, 1, 1, 4}), at(host.data(), {1, 1, 1, 1, 1, 1, 1, 40000, 4}), at(r, {1, 1, 1, 1, 1, 1, 1, 40000, 4})); },
+        [&] { dev.indexSelect(at(host.data(), {4, 4}), at(r, {100000, 4}), tensor(host.data(), {100000}, DataType::kInt32), 0); },
+        [&] { dev.indexAdd(at(host.data(), {100000, 4}), at(r, {4, 4}), tensor(host.data(), {100000}, DataType::kInt32), 0); },
+        [&] { dev.matmulEpilogue(at(host.data(), {4, 4}), at(host.data(), {4, 40000}), {}, at(r, {4, 40000})); },
+        [&] { dev.attention(at(host.data(), {1, 1, 1, 4}), at(host.data(), {1, 1, 40000, 4}), at(host.data(), {1, 1, 40000, 4}), {}, at(r, {1, 1, 1, 4}), nullptr); },
+    };
+    for (const auto& call : pairs) {
+        stub_set_budget(ctx, SIZE_MAX);
+        dev.synchronize();
+        dev.emptyCache();
+        void* idle = dev.allocate(size_t(4) << 20);
+        dev.deallocate(idle);
+        dev.synchronize();
+        stub_set_budget(ctx, stub_held(ctx) + 4096);
+        const uint64_t syncs = stub_syncs(ctx);
+        call();
+        CHECK(stub_syncs(ctx) > syncs);
+        CHECK(stub_dead_operands(ctx) == 0);
+    }
+    stub_set_budget(ctx, SIZE_MAX);
+    dev.deallocate(r);
+    dev.synchronize();
+    dev.emptyCache();
+    CHECK(stub_held(ctx) == 0);
+}
+
 static void test_destruction_returns_everything()
 {
     const long long before = stub_held_everywhere();
@@ -570,6 +634,7 @@ int main(int argc, char** argv)
     test_fills_do_not_land_behind_calls_that_wait();
     test_the_pool_is_trimmed_to_the_cache_limit();
     test_blocks_of_a_captured_step_stay_with_the_graph();
+    test_copies_of_host_operands_outlive_an_out_of_memory_retry();
     test_destruction_returns_everything();
     for (unsigned seed = 1; seed <= 4; ++seed) stress(seed, 20000);
     for (unsigned seed = 21; seed <= 24; ++seed) planner_traffic(seed, 3000);
