@@ -550,9 +550,9 @@ static void test_copies_of_host_operands_outlive_an_out_of_memory_retry()
 {
     DeviceHIP dev;
     aixk_ctx* ctx = dev.kernelContext();
-    std::vector<float> host(1 << 18, 1.5f);
+    std::vector<float> host(1 << 19, 1.5f);
     std::vector<int32_t> ints(64, 0);
-    float* r = (float*)dev.allocate(sizeof(float) << 18);
+    float* r = (float*)dev.allocate(sizeof(float) << 19);
     auto at = [&](void* p, std::vector<size_t> shape) { return tensor(p, std::move(shape)); };
     const auto h4 = at(host.data(), {2, 2, 4, 8}), r4 = at(r, {2, 2, 4, 8}), lse = at(r + 256, {2, 2, 4}), h2 = at(host.data(), {8, 8}), r2 = at(r, {8, 8}), s2 = at(r + 256, {8, 8});
     const auto lengths = tensor(ints.data(), {2}, DataType::kInt32), positions = tensor(ints.data(), {2, 4}, DataType::kInt32);
@@ -589,7 +589,7 @@ static void test_copies_of_host_operands_outlive_an_out_of_memory_retry()
         stub_set_budget(ctx, SIZE_MAX);
         dev.synchronize();
         dev.emptyCache();
-        void* idle = dev.allocate(size_t(4) << 20);
+        void* idle = dev.allocate(size_t(8) << 20);
         dev.deallocate(idle);
         dev.synchronize();
         stub_set_budget(ctx, stub_held(ctx) + 4096);
