@@ -252,14 +252,40 @@ inline uint64_t view_extent(const aixhip_tensor* t)
     return last + 1;
 }
 
-// Two views may share memory: their extents in bytes meet.
+// Views that repeat every `period` bytes lie side by side within it (the queries, keys and values of a packed projection): every
+// step of theirs is a whole number of periods or stays inside one, and what they cover of a period does not meet.
+inline bool interleaved(const aixhip_tensor* a, const aixhip_tensor* b, uint64_t period)
+{
+    uint64_t span[2];
+    const aixhip_tensor* views[2] = {a, b};
+    for (int n = 0; n < 2; ++n) {
+        const uint64_t e = aixk_dtype_size(views[n]->dtype);
+        span[n] = e;
+        for (int d = 0; d < views[n]->rank; ++d) {
+            const uint64_t step = views[n]->strides[d] * e;
+            if (views[n]->shape[d] <= 1 || step % period == 0) continue;
+            if (step > period) return false;
+            span[n] += (views[n]->shape[d] - 1) * step;
+        }
+        if (span[n] > period) return false;
+    }
+    const uintptr_t a0 = (uintptr_t)a->data + a->offset * aixk_dtype_size(a->dtype), b0 = (uintptr_t)b->data + b->offset * aixk_dtype_size(b->dtype);
+    const uint64_t between = b0 >= a0 ? (b0 - a0) % period : (period - (a0 - b0) % period) % period;
+    return between >= span[0] && between + span[1] <= period;
+}
+
+// Two views may share memory: their extents in bytes meet, and nothing shows that they only lie in between one another.
 inline bool overlap(const aixhip_tensor* a, const aixhip_tensor* b)
 {
     if (!a || !b || numel(a) == 0 || numel(b) == 0) return false;
     const size_t ea = aixk_dtype_size(a->dtype), eb = aixk_dtype_size(b->dtype);
     const char *a0 = (const char*)a->data + a->offset * ea, *a1 = (const char*)a->data + view_extent(a) * ea;
     const char *b0 = (const char*)b->data + b->offset * eb, *b1 = (const char*)b->data + view_extent(b) * eb;
-    return a0 < b1 && b0 < a1;
+    if (!(a0 < b1 && b0 < a1)) return false;
+    for (const aixhip_tensor* t : {a, b})
+        for (int d = 0; d < t->rank; ++d)
+            if (t->shape[d] > 1 && t->strides[d] > 0 && interleaved(a, b, t->strides[d] * aixk_dtype_size(t->dtype))) return false;
+    return true;
 }
 
 inline unsigned grid_for(uint64_t work_items, unsigned per_block, unsigned max_blocks)

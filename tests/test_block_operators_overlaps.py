@@ -1,0 +1,84 @@
+"""Which results of the transformer-block operators may lie in between their operands and one another, and which may not.  The
+checks end before the device is touched: a valid call gets as far as its missing context."""
+import pytest
+
+from aix_amd import kernels as K
+
+from test_block_operators_refusals import At, attention_parts, call_attention, call_rotary, refused
+
+FINE = "null context"
+
+
+def packed(at, dtype, batch, length, *heads, d=64, gap=0, order="row"):
+    """Views [batch, heads, length, d] side by side in the rows of one projection."""
+    base = at(dtype, 1)
+    width, views, offset = sum(heads) * d + gap, [], 0
+    strides = {"row": (length * width, d, width, 1), "turned": (width, d, batch * width, 1)}[order]
+    for h in heads:
+        views.append(K.tensor(base.data, dtype, (batch, h, length, d), strides, offset))
+        offset += h * d
+    return views
+
+
+def rotary(**parts):
+    spec = {"spec": True, "dims": 32, "interleaved": 0, "inverse": 0, "scaling": 0, "base": 1e4, "factor": 1.0, "original_length": 1.0, "low_turns": 0.0, "high_turns": 1.0,
+            "magnitude": 1.0}
+    return lambda: call_rotary({**spec, **parts})
+
+
+@pytest.mark.parametrize("order", ["row", "turned"])
+@pytest.mark.parametrize("heads", [(4, 4, 4), (8, 2, 2), (1, 1, 1)])
+@pytest.mark.parametrize("batch,length", [(2, 5), (1, 5), (3, 1), (1, 1)])
+def test_queries_and_keys_of_a_packed_projection_turn_in_place(order, heads, batch, length):
+    at = At()
+    q, k, v = packed(at, K.BF16, batch, length, *heads, gap=8, order=order)
+    positions = at(K.I32, batch, length)
+    refused(rotary(q=q, k=k, positions=positions, q_out=q, k_out=k), FINE)
+    if heads[0] == heads[2]:
+        refused(rotary(q=q, k=k, positions=positions, q_out=v, k_out=k), FINE)
+    if heads[1] == heads[2]:
+        refused(rotary(q=q, k=k, positions=positions, q_out=q, k_out=v), FINE)
+
+
+def test_results_in_between_the_operands_of_attention():
+    at, good = attention_parts(False)
+    q, k, v, out = packed(at, K.BF16, 2, 7, 4, 2, 2, 4)
+    refused(lambda: call_attention({**good, "q": q, "k": k, "v": v, "out": out, "lse": at(K.F32, 2, 4, 7)}), FINE)
+    refused(lambda: call_attention({**good, "q": q, "k": k, "v": v, "out": q, "lse": at(K.F32, 2, 4, 7)}), "overlaps")
+    moved = K.tensor(q.data, K.BF16, (2, 4, 7, 64), list(q.strides[:4]), 8)
+    refused(lambda: call_attention({**good, "q": q, "k": k, "v": v, "out": moved, "lse": at(K.F32, 2, 4, 7)}), "overlaps")
+    refused(rotary(q=q, k=None, positions=at(K.I32, 2, 7), q_out=moved, k_out=None), "overlaps")
+
+
+def cells(t):
+    """The element positions of a view."""
+    got = [int(t.offset)]
+    for d in range(t.rank):
+        got = [p + n * int(t.strides[d]) for p in got for n in range(int(t.shape[d]))]
+    return got
+
+
+def test_whatever_shares_an_element_is_refused():
+    """Random views of one piece of memory: a call with a result and an operand that share an element is never let through."""
+    import random
+    rng, at, apart = random.Random(5), At(), 0
+    positions = at(K.I32, 2, 3)
+    base = at(K.F32, 1)
+    for _ in range(4000):
+        views = []
+        for _ in range(2):
+            dims, strides, run = rng.sample(range(4), 4), [0] * 4, 1
+            shape = (2, 2, 3, 4)
+            for d in dims:
+                strides[d], run = run, run * shape[d] * rng.choice((1, 1, 1, 2, 3)) + rng.choice((0, 0, 4, 8))
+            views.append(K.tensor(base.data, K.F32, shape, strides, rng.choice((0, 4, 8, 16, rng.randrange(64)))))
+        q, out = views
+        first, second = set(cells(q)), cells(out)
+        assert rotary(q=q, k=None, positions=positions, q_out=out, k_out=None, dims=4)() == 1
+        text = K.load().aixk_last_error().decode()
+        same = q.offset == out.offset and list(q.strides[:4]) == list(out.strides[:4])
+        if same or "overlaps" not in text:
+            assert same or not first & set(second), (list(q.strides[:4]), q.offset, list(out.strides[:4]), out.offset)
+            assert FINE in text
+            apart += not same
+    assert apart                                             # (the rule lets some through: those that it can show to be apart)
