@@ -50,6 +50,31 @@ def test_results_in_between_the_operands_of_attention():
     refused(rotary(q=q, k=None, positions=at(K.I32, 2, 7), q_out=moved, k_out=None), "overlaps")
 
 
+@pytest.mark.parametrize("first,second", [("dq", "dk"), ("dq", "dv"), ("dk", "dv")])
+@pytest.mark.parametrize("offset", [0, 1, 64, 300])
+def test_gradients_that_share_memory_are_refused(first, second, offset):
+    at, good = attention_parts(True)
+    shape = tuple(good[second].shape[:4])
+    refused(lambda: call_attention({**good, second: K.tensor(good[first].data, K.BF16, shape, None, offset)}), "share")
+    refused(lambda: call_attention({**good, first: K.tensor(good[second].data, K.BF16, tuple(good[first].shape[:4]), None, offset)}), "share")
+
+
+def test_gradients_side_by_side():
+    at, good = attention_parts(True)
+    dq, dk, dv = packed(at, K.BF16, 2, 7, 4, 2, 2)
+    like_q = {n: at(K.BF16, 2, 4, 7, 64) for n in ("q", "grad", "out")}
+    refused(lambda: call_attention({**good, **like_q, "lse": at(K.F32, 2, 4, 7), "dq": dq, "dk": dk, "dv": dv}), FINE)
+    dv.offset += 4
+    refused(lambda: call_attention({**good, **like_q, "lse": at(K.F32, 2, 4, 7), "dq": dq, "dk": dk, "dv": dv}), "share")     # (its last elements: the next row's first)
+
+
+@pytest.mark.parametrize("offset", [0, 1, 64])
+def test_turned_queries_and_keys_that_share_memory_are_refused(offset):
+    at = At()
+    q, k, positions, q_out = at(K.F32, 2, 4, 5, 64), at(K.F32, 2, 2, 5, 64), at(K.I32, 2, 5), at(K.F32, 2, 4, 5, 64)
+    refused(rotary(q=q, k=k, positions=positions, q_out=q_out, k_out=K.tensor(q_out.data, K.F32, (2, 2, 5, 64), None, offset)), "share")
+
+
 def cells(t):
     """The element positions of a view."""
     got = [int(t.offset)]
