@@ -68,6 +68,7 @@ struct Call {
             AIXK_REQUIRE(t->shape[d] == like->shape[d], "%s: the shape of %s does not match the operands", what, name);
             AIXK_REQUIRE(t->size == 0 || t->shape[d] <= 1 || t->strides[d] != 0, "%s: %s cannot be a broadcast view", what, name);
         }
+        AIXK_REQUIRE(distinct(t), "%s: %s meets an element twice", what, name);
         *out_view = view(t);
         const size_t e = aixk_dtype_size(dtype);
         bool w = (t->strides[3] == 1 || t->shape[3] == 1) && t->shape[3] % 4 == 0 && (uintptr_t)out_view->p % (4 * e) == 0;

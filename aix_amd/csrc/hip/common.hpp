@@ -252,6 +252,27 @@ inline uint64_t view_extent(const aixhip_tensor* t)
     return last + 1;
 }
 
+// A view that meets no element twice, as far as its strides show it: from the smallest stride up, each steps over everything that
+// the smaller ones reach.  (So do slices and permutations of a dense tensor.)
+inline bool distinct(const aixhip_tensor* t)
+{
+    uint64_t reach = 0, from = 0;                              // positions up to `reach` by the strides below `from`
+    if (numel(t) == 0) return true;
+    for (int taken = 0; taken < t->rank; ++taken) {
+        int next = -1;
+        for (int d = 0; d < t->rank; ++d) {
+            if (t->shape[d] <= 1 || t->strides[d] < from) continue;
+            if (next < 0 || t->strides[d] < t->strides[next]) next = d;
+        }
+        if (next < 0) break;
+        if (t->strides[next] <= reach) return false;           // (a stride of 0, or one that two dims share, among them)
+        reach += (t->shape[next] - 1) * t->strides[next];
+        from = t->strides[next] + 1;
+        for (int d = 0; d < t->rank; ++d) if (d != next && t->shape[d] > 1 && t->strides[d] == t->strides[next]) return false;
+    }
+    return true;
+}
+
 // Views that repeat every `period` bytes lie side by side within it (the queries, keys and values of a packed projection): every
 // step of theirs is a whole number of periods or stays inside one, and what they cover of a period does not meet.
 inline bool interleaved(const aixhip_tensor* a, const aixhip_tensor* b, uint64_t period)

@@ -154,6 +154,7 @@ int check_pair(const aixhip_tensor* in, const aixhip_tensor* out, const char* na
         AIXK_REQUIRE(out->shape[d] == in->shape[d], "rotary: the shape of the result for %s differs", name);
         AIXK_REQUIRE(out->size == 0 || out->shape[d] <= 1 || out->strides[d] != 0, "rotary: the result for %s cannot be a broadcast view", name);
     }
+    AIXK_REQUIRE(distinct(out), "rotary: the result for %s meets an element twice", name);
     return AIXK_OK;
 }
 

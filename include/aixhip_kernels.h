@@ -230,9 +230,10 @@ int32_t aixk_matmul_grouped(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_
 /* ---- operators of transformer blocks (no counterpart in the reference, which composes them from the operators above) ---- */
 /* What these share: element types f32, f16 and bf16 (one per call), sums, softmax statistics and norms in f32, one rounding
  * per result unless stated.  Operands are any views; results are addressed through their offset and strides (like
- * aixk_slice_set's), may not be broadcast views and may not overlap one another, nor an operand unless stated; lying in between
- * another view's elements, as the parts of a packed projection do, is no overlap.  Operand and result memory may be any device memory of the
- * context's GPU whose earlier use the caller has ordered before the context's stream.
+ * aixk_slice_set's), which have to be those of a slice or permutation of a dense tensor: no element may be met twice.  Results may
+ * not overlap one another, nor an operand unless stated; lying in between another view's elements, as the parts of a packed
+ * projection do, is no overlap.  Operand and result memory may be any device memory of the context's GPU whose earlier use the
+ * caller has ordered before the context's stream.
  * The calls allocate nothing but workspaces of the context that grow on demand (inside a capture: AIXK_EINVAL if one would
  * have to grow; run the same call once before). */
 

@@ -75,6 +75,30 @@ def test_turned_queries_and_keys_that_share_memory_are_refused(offset):
     refused(rotary(q=q, k=k, positions=positions, q_out=q_out, k_out=K.tensor(q_out.data, K.F32, (2, 2, 5, 64), None, offset)), "share")
 
 
+@pytest.mark.parametrize("strides", [(1280, 320, 1, 1), (1280, 63, 252, 1), (64, 1280, 64, 1), (1280, 320, 64, 2), (1280, 64, 200, 1)])
+def test_results_that_meet_an_element_twice_are_refused(strides):
+    at, good = attention_parts(False)
+    refused(lambda: call_attention({**good, "out": at(K.BF16, 2, 4, 5, 64, strides=strides)}), "twice")
+    at, good = attention_parts(True)
+    for name in ("dq", "dk", "dv"):
+        refused(lambda: call_attention({**good, name: at(K.BF16, *good[name].shape[:4], strides=strides)}), "twice")
+    q, k, positions = at(K.F32, 2, 4, 5, 64), at(K.F32, 2, 4, 5, 64), at(K.I32, 2, 5)
+    refused(rotary(q=q, k=k, positions=positions, q_out=at(K.F32, 2, 4, 5, 64, strides=strides), k_out=k), "twice")
+    refused(rotary(q=q, k=k, positions=positions, q_out=q, k_out=at(K.F32, 2, 4, 5, 64, strides=strides)), "twice")
+
+
+@pytest.mark.parametrize("shape,strides", [((2, 4, 5, 64), (1280, 64, 256, 1)), ((2, 4, 5, 64), (1, 2, 512, 8)), ((2, 4, 5, 64), (10 ** 6, 10 ** 5, 10 ** 4, 3)),
+                                           ((1, 4, 5, 64), (0, 320, 64, 1)), ((2, 4, 1, 64), (256, 64, 1, 1)), ((2, 4, 5, 1), (20, 5, 1, 0))])
+def test_results_of_any_order(shape, strides):
+    at = At()
+    q = at(K.BF16, *shape)
+    refused(rotary(q=q, k=None, positions=at(K.I32, shape[0], shape[2]), q_out=at(K.BF16, *shape, strides=strides), k_out=None, dims=2 if shape[3] > 1 else 0),
+            FINE if shape[3] > 1 else "turned part")
+    k = at(K.BF16, shape[0], shape[1], 7, shape[3])
+    parts = {"q": q, "k": k, "v": at(K.BF16, *k.shape[:4]), "out": at(K.BF16, *shape, strides=strides), "lse": None, "lengths": None, "starts": None, "scale": 1.0, "spec": True}
+    refused(lambda: call_attention(parts), FINE)
+
+
 def cells(t):
     """The element positions of a view."""
     got = [int(t.offset)]
