@@ -37,7 +37,8 @@ struct Call {
         AIXK_REQUIRE(tq->shape[0] < (1u << 20) && tq->shape[1] < (1u << 20) && tq->shape[0] * tq->shape[1] < (1u << 28), "%s: too many sequences or heads", what);
         AIXK_REQUIRE((tk->shape[1] > 0 || tq->shape[1] == 0) && (tk->shape[1] == 0 || tq->shape[1] % tk->shape[1] == 0),
                      "%s: the heads of the queries must be a multiple of those of the keys", what);
-        AIXK_REQUIRE(std::isfinite(spec->scale) && spec->scale > 0.0f, "%s: the scale must be a positive number", what);
+        // (the kernels' exponentials are powers of two: a factor beyond f32 would turn a score of zero into a NaN)
+        AIXK_REQUIRE(std::isfinite(spec->scale * kLog2e) && spec->scale > 0.0f, "%s: the scale must be a positive number, at most 2^127", what);
         s.B = (u32)tq->shape[0]; s.H = (u32)tq->shape[1]; s.HK = (u32)tk->shape[1]; s.G = s.HK ? s.H / s.HK : 0;
         s.SQ = (i32)tq->shape[2]; s.SK = (i32)tk->shape[2];
         s.D = (u32)tq->shape[3];

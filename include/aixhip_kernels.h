@@ -246,7 +246,7 @@ int32_t aixk_matmul_grouped(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_
  * front of a length take part in the products with a weight of zero: keys and values there, queries and their gradients must be
  * finite (their scores need not be). */
 typedef struct aixk_attention_spec {
-    float    scale;                  /* factor of the scores, positive and finite */
+    float    scale;                  /* factor of the scores, positive, at most 2^127 */
     int32_t  causal;
     uint64_t window;                 /* 0: none */
     uint64_t sinks;                  /* leading keys that a window does not hide */
