@@ -473,15 +473,15 @@ __global__ __launch_bounds__(WAVES * 64) void attention_split_k(SplitArgs a)
         float top = -__builtin_inff();
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ml[(w * 16 + row) * 2]);
+        // (no maximum: a row without a visible key, whose sums are zeros, or one of NaN scores, whose sums are NaNs and stay so)
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
         f32x4 sum = f32x4{};
         float total = 0.0f;
-        if (top != -__builtin_inff()) {
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                const float f = exp2_of(ml[(w * 16 + row) * 2] - top);
-                total += f * ml[(w * 16 + row) * 2 + 1];
-                sum += f * *(const f32x4*)(all + (w * 16 + row) * DP + (d ^ (4 * (row & 7))));
-            }
+        for (int w = 0; w < WAVES; ++w) {
+            const float f = exp2_of(ml[(w * 16 + row) * 2] - ref);
+            total += f * ml[(w * 16 + row) * 2 + 1];
+            sum += f * *(const f32x4*)(all + (w * 16 + row) * DP + (d ^ (4 * (row & 7))));
         }
         const u32 qi = (r0 + row) % (u32)s.SQ, qh = hk * s.G + (r0 + row) / (u32)s.SQ;
         const u64 at = ((u64)b * s.H + qh) * (u32)s.SQ + qi;
@@ -510,17 +510,16 @@ __global__ __launch_bounds__(256) void attention_join_k(SplitArgs a)
     float top = -__builtin_inff(), total = 0.0f;
 #pragma unroll 8
     for (u32 k = 0; k < a.splits; ++k) top = fmaxf(top, a.part_ml[(k * rows + at) * 2]);
+    const float ref = top == -__builtin_inff() ? 0.0f : top;       // as where the waves' shares meet
     f32x4 sum = f32x4{};
-    if (top != -__builtin_inff()) {
 #pragma unroll 8
-        for (u32 k = 0; k < a.splits; ++k) {
-            const f32x2 ml = *(const f32x2*)(a.part_ml + (k * rows + at) * 2);
-            total += exp2_of(ml.x - top) * ml.y;
-        }
-#pragma unroll 2
-        for (u32 k = group; k < a.splits; k += GROUPS)
-            sum += exp2_of(a.part_ml[(k * rows + at) * 2] - top) * *(const f32x4*)(a.part_o + (k * rows + at) * DP + d);
+    for (u32 k = 0; k < a.splits; ++k) {
+        const f32x2 ml = *(const f32x2*)(a.part_ml + (k * rows + at) * 2);
+        total += exp2_of(ml.x - ref) * ml.y;
     }
+#pragma unroll 2
+    for (u32 k = group; k < a.splits; k += GROUPS)
+        sum += exp2_of(a.part_ml[(k * rows + at) * 2] - ref) * *(const f32x4*)(a.part_o + (k * rows + at) * DP + d);
     part[group][lane] = sum;
     __syncthreads();
     if (group) return;
