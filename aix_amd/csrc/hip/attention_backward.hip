@@ -30,9 +30,50 @@ struct BackwardArgs {
                                               // follow, [share][dk, dv][batch * key heads * lead_keys][DP] (see share_of)
 };
 
+// P and dS are rounded to the operands' type to feed the matrix unit.  bf16 has the range of f32; f16 holds 2^-24 to 65504, and dS
+// has no such bounds: loss-scaled gradients on a peaked row pass the upper end, an even row over some thousand keys the lower.  So
+// for f16 a lane (a query in attention_dq_k, a key in attention_dkdv_k) has its dS, and its sums, times a power of two of its own: 2^75
+// at first, which no product of f16 numbers takes out of f32, and lowered when a tile's largest passes 2^15, so that it comes to
+// 2^11 .. 2^12.  What is left of the range below is 2^-36 of the lane's largest dS.  P is at most 1 and has 2^15.  (The factor
+// enters with the exponential's argument where that is dS's alone.  Looking for the largest costs f16 11 %: 16 x 12 heads of 512 x 64,
+// window 128, 57.4 us where bf16 takes 50.7; 16 heads on 4 of 4096 x 128, window 1024, 200 and 179; 21 % at 256 dims.)
+template <class T> struct Unit {
+    static constexpr int kProbability = 0;
+    __device__ __forceinline__ float in_exponent(float lse2) const { return lse2; }
+    __device__ __forceinline__ float times(float x) const { return x; }
+    template <int DB> __device__ __forceinline__ void fit(float*, f32x16 (&)[DB]) {}
+    __device__ __forceinline__ float taken_out(float x) const { return x; }
+};
+template <> struct Unit<f16> {
+    static constexpr int kProbability = 15;
+    int exponent = 75;
+    __device__ __forceinline__ float in_exponent(float lse2) const { return lse2 - (float)exponent; }
+    __device__ __forceinline__ float times(float x) const { return x * __builtin_amdgcn_ldexpf(1.0f, exponent - kProbability); }      // of x with P's factor
+    // a tile of one query's or key's dS, half of it in this lane, and its sums so far
+    template <int DB> __device__ __forceinline__ void fit(float* e, f32x16 (&sums)[DB])
+    {
+        float top = fabsf(e[0]);
+#pragma unroll
+        for (int v = 1; v < 16; ++v) top = fmaxf(top, fabsf(e[v]));
+        if (!__any(top > 32768.0f)) return;
+        top = max_of_halves(top);
+        int lower = top > 32768.0f ? 12 - __builtin_amdgcn_frexp_expf(top) : 0;
+        lower = lower < 0 ? lower : 0;                         // (an infinity has no exponent)
+        exponent += lower;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) e[v] = __builtin_amdgcn_ldexpf(e[v], lower);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sums[d][v] = __builtin_amdgcn_ldexpf(sums[d][v], lower);
+    }
+    __device__ __forceinline__ float taken_out(float x) const { return __builtin_amdgcn_ldexpf(x, -exponent); }
+};
+
 // As in attention_k the scores are transposed (a lane = one query): dS^T, rounded, feeds dq^T = K^T dS^T as it lies.
+// (Rows of 128 bytes: three waves per SIMD, which bf16 comes to by itself; f16 at two 63.6 us for the 16 x 12 heads.)
 template <class T, int DP, int KT>
-__global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k(BackwardArgs a)
+__global__ __launch_bounds__(256, (DP * sizeof(T) == 128 ? 3 : waves_per_simd<T, DP>())) void attention_dq_k(BackwardArgs a)
 {
     typedef Mma<T> M;
     typedef typename M::Frag Frag;
@@ -85,6 +126,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
     for (int d = 0; d < DB; ++d) acc[d] = f32x16{};
 #pragma unroll
     for (int v = 0; v < 16; ++v) less[v] = -delta;
+    Unit<T> unit;
     const float c2 = s.scale * kLog2e;
 
     const Keys seen = keys_of(s, r.length, p);
@@ -120,15 +162,15 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
             }
             const bool masked = !all_visible(s, r.length, r.start + w0, r.start + w1, k0, k0 + 31);
             float e[16];
+            const float ref = unit.in_exponent(lse2);
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                e[v] = exp2_of(x[v] * c2 - lse2) * dp[v];
-            }
+            for (int v = 0; v < 16; ++v) e[v] = exp2_of(x[v] * c2 - ref) * dp[v];
             if (masked) {
                 const u32 word = seen.word(k0) >> (4 * half);
 #pragma unroll
                 for (int v = 0; v < 16; ++v) e[v] = drop(e[v], word, 8 * (v >> 2) + (v & 3));
             }
+            unit.fit(e, acc);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const Frag ds = M::pack8(e + 8 * c);
@@ -139,6 +181,10 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP>())) void attention_dq_k
     }
     if (!on) return;
     char* row = a.dq.p + (b * a.dq.b + h * a.dq.h + (u64)(u32)i * a.dq.s) * sizeof(T);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[d][v] = unit.taken_out(acc[d][v]);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -239,6 +285,7 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
     f32x16 dk[DB], dv[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) { dk[d] = f32x16{}; dv[d] = f32x16{}; }
+    Unit<T> unit;
     const float c2 = s.scale * kLog2e;
 
     // the queries that can see a key of this block: positions [lo, hi)
@@ -296,7 +343,7 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
         __syncthreads();
         sq.store(qs, i0, s.SQ, s.DW, tid);
         sg.store(gs, i0, s.SQ, s.DW, tid);
-        if (tid < QT) { ls[tid] = i0 + tid < s.SQ && next_l != -__builtin_inff() ? next_l * kLog2e : __builtin_inff(); ds[tid] = next_d; }
+        if (tid < QT) { ls[tid] = i0 + tid < s.SQ && next_l != -__builtin_inff() ? next_l * kLog2e - Unit<T>::kProbability : __builtin_inff(); ds[tid] = next_d; }
         __syncthreads();
         if (n + 1 < to) { on_from(next); load(next); }
 #pragma unroll
@@ -318,7 +365,7 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
                     e[4 * g + v] = exp2_of(x[4 * g + v] * c2 - l4[v]);
-                    w[4 * g + v] = e[4 * g + v] * (dp[4 * g + v] - d4[v]);
+                    w[4 * g + v] = unit.times(e[4 * g + v] * (dp[4 * g + v] - d4[v]));
                 }
             }
             if (masked) {
@@ -329,6 +376,7 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
                     w[v] = drop(w[v], word, 8 * (v >> 2) + (v & 3));
                 }
             }
+            unit.fit(w, dk);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const Frag fp = M::pack8(e + 8 * c), fs = M::pack8(w + 8 * c);
@@ -340,6 +388,15 @@ __global__ __launch_bounds__((KeyBlock<T, DP>::kThreads), (KeyBlock<T, DP>::kWav
                 }
             }
         }
+    }
+    if constexpr (Unit<T>::kProbability != 0) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                dk[d][v] = unit.taken_out(dk[d][v]);
+                dv[d][v] = __builtin_amdgcn_ldexpf(dv[d][v], -Unit<T>::kProbability);
+            }
     }
     if (j >= s.SK) return;
     if (apart && split && j >= (i32)a.lead_keys) return;

@@ -260,7 +260,10 @@ typedef struct aixk_attention_spec {
 int32_t aixk_attention(aixk_ctx* ctx, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* v, const aixk_attention_spec* spec,
                        const aixhip_tensor* out, const aixhip_tensor* lse);
 /* The gradients of the above: grad and out like q, lse as aixk_attention left it; dq like q, dk and dv like k.  Key heads
- * shared by several query heads receive the sum over them.  No atomics: results repeat bit for bit. */
+ * shared by several query heads receive the sum over them.  No atomics: results repeat bit for bit.  With P = exp(scale q k^T - lse)
+ * and dS = P (grad v^T - sum_d grad out), dv = P^T grad, dq = scale dS k and dk = scale dS^T q; P and dS are rounded to the element
+ * type before these products (the matrix unit's operand type).  f16: both with a power of two that keeps them within its range,
+ * whatever finite gradients, values and lengths; dS to 2^-36 of the largest of its query (for dq) or key (for dk). */
 int32_t aixk_attention_backward(aixk_ctx* ctx, const aixhip_tensor* grad, const aixhip_tensor* q, const aixhip_tensor* k, const aixhip_tensor* v,
                                 const aixhip_tensor* out, const aixhip_tensor* lse, const aixk_attention_spec* spec,
                                 const aixhip_tensor* dq, const aixhip_tensor* dk, const aixhip_tensor* dv);
