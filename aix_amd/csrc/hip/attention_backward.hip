@@ -10,6 +10,7 @@
 #include "attention_host.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 using namespace aixd;
 using namespace aixk;
@@ -468,8 +469,8 @@ template <class T, int DP> int backward(aixk_ctx* ctx, const Call& c, BackwardAr
     const u64 heads = (u64)s.B * s.HK, rows = heads * (u32)s.SK;
     // Shares of the queries by a cost in microseconds: rounds of workgroups, each of its steps (about 2 us, three of them the
     // workgroup's own), and the shares written and read again (4 TB/s, and the joining launch).  Key tiles with leading keys, which
-    // every query sees, take as many more shares as they have more queries.  16 heads on 4 of 4096 x 128, window 1024: 3 shares
-    // 98 us and 13 for joining them, 8 shares 148 in all.
+    // every query sees, take up to as many more shares as they have more queries: they start first, so that a chip full of other
+    // work hides their longer chains.  16 heads on 4 of 4096 x 128, window 1024: 3 shares 98 us and 13 for joining them, 8 shares 148 in all.
     constexpr u64 resident = KeyBlock<T, DP>::kWaves * 256 / KeyBlock<T, DP>::kThreads;
     const u64 slots = (u64)ctx->cus * resident;
     const u64 seen = s.window && (u64)s.window + keys < (u64)(u32)s.SQ ? (u64)s.window + keys : (u64)(u32)s.SQ;      // queries of a tile at most
@@ -480,30 +481,52 @@ template <class T, int DP> int backward(aixk_ctx* ctx, const Call& c, BackwardAr
     }
     // keys with shares of their own: whole tiles if the other tiles have shares too, else the leading keys
     auto lead_keys = [&](u64 sp) { return a.lead ? std::min<u64>(sp > 1 ? (u64)a.lead * keys : (u64)(u32)s.sinks, (u64)(u32)s.SK) : 0; };
-    u64 splits = 1, planes = 0, grid = 0;
-    double least = 0.0;
-    for (u64 sp = 1; sp <= 64 && (sp == 1 || sp * 4 <= steps); ++sp) {
-        const u64 n = heads * (a.lead * sp * more + (a.tiles - a.lead) * sp);
-        const u64 shares = (sp > 1 ? sp * rows : 0) + (sp * more > 1 ? (sp > 1 ? sp * (more - 1) : more) * heads * lead_keys(sp) : 0);
-        const double cost = 2.0 * (double)((n + slots - 1) / slots) * (double)((steps + sp - 1) / sp + 3) + (shares ? 3.0 + (double)shares * (16.0 * DP / 4e6) : 0.0);
-        if (sp == 1 || cost < least) { least = cost; splits = sp; planes = shares; grid = n; }
+    struct Plan { u64 splits, more, planes, grid; };
+    // the cheapest shares whose partial sums take no more than `most` bytes (fewer on leading keys than more queries only for a twentieth:
+    // 16 x 16 heads of 8192 x 128, window 256, 1024 leading keys: 5.7 ms with one share, 7.4 with 16 of 4 GB in all; 2 x 32 heads on 8 of
+    // 8192 x 128, window 512, four leading keys, equal by this count: 767 us with 11, 788 with 6)
+    auto cheapest = [&](u64 most) {
+        Plan best{};
+        double least = -1.0;
+        for (u64 sp = 1; sp <= 64 && (sp == 1 || sp * 4 <= steps); ++sp)
+            for (u64 mo = a.lead ? more : 1;; mo = (mo + 1) / 2) {
+                const u64 n = heads * (a.lead * sp * mo + (a.tiles - a.lead) * sp);
+                const u64 shares = (sp > 1 ? sp * rows : 0) + (sp * mo > 1 ? (sp > 1 ? sp * (mo - 1) : mo) * heads * lead_keys(sp) : 0);
+                // steps of a workgroup, and of one on leading keys: all queries of theirs over its shares, or (one share for the
+                // other tiles) the first share's as anywhere and the rest over the others
+                const double chain = (double)((steps + sp - 1) / sp + 3);
+                const double reach = mo == more ? 1.0 : sp > 1 ? (double)more / (double)mo : mo > 1 ? (double)(more - 1) / (double)(mo - 1) : (double)more;
+                const double led = a.lead ? std::ceil((double)steps * reach / (double)sp) + 3.0 : chain;
+                const double full = std::ceil((double)heads * ((double)(a.lead * sp * mo) * led / chain + (double)((a.tiles - a.lead) * sp)));
+                const double cost = 2.0 * std::max(std::ceil(full / (double)slots) * chain, led) + (shares ? 3.0 + (double)shares * (16.0 * DP / 4e6) : 0.0);
+                if (shares * 2 * DP * sizeof(float) <= most && (least < 0.0 || cost < least * (mo == more ? 1.0 : 0.95))) { least = cost; best = Plan{sp, mo, shares, n}; }
+                if (mo == 1) break;
+            }
+        return best;
+    };
+    // At most as much as the gradients in f32, or 256 MB: many leading keys on many heads came to 16 GB (4 x 32 heads of 16384 x 128,
+    // window 1024, 4096 leading keys), though every head's own tiles fill the chip.  Without that memory: no shares.
+    const u64 gradients = rows * 2 * DP * sizeof(float);
+    void* ws = nullptr;
+    Plan plan = cheapest(std::max<u64>(u64(256) << 20, gradients));
+    if (plan.planes) {
+        int rc = block_scratch(ctx, kScratchParts, (size_t)plan.planes * 2 * DP * sizeof(float), &ws);
+        if (rc == AIXK_ENOMEM) { plan = cheapest(0); rc = AIXK_OK; ws = nullptr; }
+        AIXK_TRY(rc);
     }
-    a.splits = (u32)splits;
-    a.lead_keys = (u32)lead_keys(splits);
-    a.lead_splits = (u32)(a.lead ? splits * more : splits);
+    a.splits = (u32)plan.splits;
+    a.lead_keys = (u32)lead_keys(plan.splits);
+    a.lead_splits = (u32)(a.lead ? plan.splits * plan.more : plan.splits);
+    a.part = (float*)ws;
+    const u64 grid = plan.grid;
     AIXK_REQUIRE(grid < (1ull << 31), "attention_backward: too many rows");
-    if (planes) {
-        void* ws;
-        AIXK_TRY(block_scratch(ctx, kScratchParts, (size_t)planes * 2 * DP * sizeof(float), &ws));
-        a.part = (float*)ws;
-    }
     constexpr size_t lds = KeyBlock<T, DP>::kLds;
     AIXK_TRY(allow_lds(attention_dkdv_k<T, DP>, lds));
     hipLaunchKernelGGL((attention_dkdv_k<T, DP>), dim3((unsigned)grid), dim3(KeyBlock<T, DP>::kThreads), lds, ctx->stream, a);
     AIXK_HIP(hipGetLastError());
     if (a.part) {
         constexpr u32 per = 256 / (DP / 4);
-        const u64 joined = heads * (splits > 1 ? (u64)(u32)s.SK : a.lead_keys);
+        const u64 joined = heads * (plan.splits > 1 ? (u64)(u32)s.SK : a.lead_keys);
         hipLaunchKernelGGL((attention_dkdv_join_k<T, DP>), dim3((unsigned)((joined + per - 1) / per)), dim3(256), 0, ctx->stream, a);
         AIXK_HIP(hipGetLastError());
     }
