@@ -18,6 +18,11 @@ inline BlockOperators& blockOperators(Device* dev)
     return *ops;
 }
 
+inline void requireRank(const Tensor& t, size_t rank, const char* what)
+{
+    if (t.shape().size() != rank) throw std::invalid_argument(what);
+}
+
 // [batch, heads, sequence, head dim] over memory [batch, sequence, heads, head dim]: what projections leave and take
 inline Value headsOf(Device* dev, DataType dt, const Shape& s) { return Value(dev, dt, Shape{s[0], s[2], s[1], s[3]}).transpose(1, 2); }
 
@@ -36,6 +41,7 @@ struct AttentionMask {
 // q [batch, heads, queries, d], k and v [batch, key heads, keys, d] -> like q
 inline Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const AttentionMask& mask)
 {
+    for (const Tensor* t : {&q, &k, &v}) requireRank(*t, 4, "attention: queries, keys and values must be [batch, heads, sequence, head dim]");
     Device* dev = q.device();
     const Shape& s = q.shape();
     const Value out = headsOf(dev, q.dtype(), s), lse(dev, DataType::kFloat32, Shape{s[0], s[1], s[2]});
@@ -55,6 +61,7 @@ inline Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const
 // queries and keys turned by their positions (int32 [batch, sequence]), in one call
 inline std::pair<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const Value& positions, const aix::hip::RotarySpec& spec)
 {
+    for (const Tensor* t : {&q, &k}) requireRank(*t, 4, "rotary: queries and keys must be [batch, heads, sequence, head dim]");
     Device* dev = q.device();
     const Value tq = headsOf(dev, q.dtype(), q.shape()), tk = headsOf(dev, k.dtype(), k.shape());
     blockOperators(dev).rotary(q.value().params(), &k.value().params(), positions.params(), spec, tq.params(), &tk.params());
@@ -72,6 +79,7 @@ inline std::pair<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const 
 // act(x . w + b) [+ residual]: x [rows, in], w [in, out], b [1, out]
 inline Tensor linear(const Tensor& x, const Tensor& w, const Tensor& b, Activation act = Activation::kNone, const Tensor* residual = nullptr)
 {
+    for (const Tensor* t : {&x, &w}) requireRank(*t, 2, "linear: rows and weights must be 2-D");
     Device* dev = x.device();
     const Shape s{x.shape()[0], w.shape()[1]};
     const Value out(dev, x.dtype(), s), pre = act != Activation::kNone ? Value(dev, x.dtype(), s) : Value();

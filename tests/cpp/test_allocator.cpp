@@ -4,6 +4,7 @@
 // reference's sanitizer configurations (CMakeLists.txt:25, 47-53).
 // Deferred-free semantics follow aixDeviceMetal.cpp:251-259, 1352-1377; out-of-memory retry :1455-1471.
 #include "device/device_hip.hpp"
+#include "frontend/blocks.hpp"
 #include "aixhip_kernels.h"
 
 #include <algorithm>
@@ -605,6 +606,33 @@ static void test_copies_of_host_operands_outlive_an_out_of_memory_retry()
     CHECK(stub_held(ctx) == 0);
 }
 
+// The transformer-block operators of the front-end look at their operands' ranks before they take shapes apart.
+static void test_operands_of_another_rank_are_refused()
+{
+    DeviceHIP dev;
+    auto of = [&](aixfe::Shape s) { return aixfe::Tensor(aixfe::Value(&dev, DataType::kFloat32, std::move(s))); };
+    const auto heads = of({2, 2, 4, 8}), flat = of({2, 8}), line = of({8}), three = of({2, 4, 8}), square = of({8, 8}), bias = of({1, 8});
+    const aixfe::AttentionMask mask;
+    const aixfe::Value positions(&dev, DataType::kInt32, aixfe::Shape{2, 4});
+    aix::hip::RotarySpec turn;
+    turn.dims = 8;
+    for (const auto* t : {&flat, &line, &three}) {
+        CHECK(throws<std::invalid_argument>([&] { aixfe::attention(*t, heads, heads, mask); }));
+        CHECK(throws<std::invalid_argument>([&] { aixfe::attention(heads, *t, heads, mask); }));
+        CHECK(throws<std::invalid_argument>([&] { aixfe::attention(heads, heads, *t, mask); }));
+        CHECK(throws<std::invalid_argument>([&] { aixfe::rotary(*t, heads, positions, turn); }));
+        CHECK(throws<std::invalid_argument>([&] { aixfe::rotary(heads, *t, positions, turn); }));
+    }
+    for (const auto* t : {&line, &three, &heads}) {
+        CHECK(throws<std::invalid_argument>([&] { aixfe::linear(*t, square, bias); }));
+        CHECK(throws<std::invalid_argument>([&] { aixfe::linear(flat, *t, bias); }));
+    }
+    CHECK(aixfe::attention(heads, heads, heads, mask).shape() == heads.shape());
+    CHECK(aixfe::rotary(heads, heads, positions, turn).first.shape() == heads.shape());
+    CHECK(aixfe::linear(flat, square, bias).shape() == flat.shape());
+    dev.synchronize();
+}
+
 static void test_destruction_returns_everything()
 {
     const long long before = stub_held_everywhere();
@@ -635,6 +663,7 @@ int main(int argc, char** argv)
     test_the_pool_is_trimmed_to_the_cache_limit();
     test_blocks_of_a_captured_step_stay_with_the_graph();
     test_copies_of_host_operands_outlive_an_out_of_memory_retry();
+    test_operands_of_another_rank_are_refused();
     test_destruction_returns_everything();
     for (unsigned seed = 1; seed <= 4; ++seed) stress(seed, 20000);
     for (unsigned seed = 21; seed <= 24; ++seed) planner_traffic(seed, 3000);
