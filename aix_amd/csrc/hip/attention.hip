@@ -607,17 +607,31 @@ int pack(aixk_ctx* ctx, int dtype, const View& src, void* dst, u32 B, u32 H, u64
 
 namespace {
 
+// Microseconds of the two ways, by bytes per element and padded head dim: a workgroup's launch and ends and each of its steps of 64
+// keys; the two launches of shares and each step of 16 rows and 32 keys for every wave of (up to) two workgroups per compute unit.  Fitted to both, each
+// forced, on 8 heads of n x n (256, 512), n x 1024 (64, 128), 256 x 2048 and 1024 x 4096, 32 on 8 of 128 and 256 x 8192 and 12 of 40 x 512:
+// the choice is the faster one or within 10 % of it there.  Split / not, us:
+//                       16-bit, 64    128         256        f32, 64     128         256
+//   8 of 512 x 512      16.5 / 10.6   20.4 / 16.1  51 / 45   23 / 29     41 / 48     62 / 97
+//   8 of 1024 x 4096    56.9 / 56.9   92 / 94     441 / 306  135 / 200   400 / 351   820 / 724
+//   32 on 8, 128 x 8192   52 / 108    89 / 182    449 / 603  129 / 394   402 / 698   897 / 1440
+//   32 on 8, 256 x 8192   90 / 108   160 / 182    808 / 603  235 / 395   717 / 698  1729 / 1443
+template <size_t BYTES, int DP> struct SplitOrNot;
+template <> struct SplitOrNot<2, 64>  { static constexpr double block = 3.8, block_step = 0.82, split = 8.0, split_step = 1.4; };
+template <> struct SplitOrNot<2, 128> { static constexpr double block = 5.0, block_step = 1.38, split = 12.0, split_step = 2.45; };
+template <> struct SplitOrNot<2, 256> { static constexpr double block = 8.0, block_step = 4.65, split = 22.0, split_step = 12.4; };
+template <> struct SplitOrNot<4, 64>  { static constexpr double block = 4.5, block_step = 3.04, split = 10.0, split_step = 3.6; };
+template <> struct SplitOrNot<4, 128> { static constexpr double block = 5.0, block_step = 5.41, split = 15.0, split_step = 11.2; };
+template <> struct SplitOrNot<4, 256> { static constexpr double block = 6.0, block_step = 11.2, split = 15.0, split_step = 13.2; };
+
 template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
 {
     const Shape& s = c.s;
     const u64 rows = (u64)s.B * s.H * (u32)s.SQ;
     const u64 R = (u64)s.G * (u32)s.SQ;
     const u64 wide = (u64)s.B * s.H * (((u32)s.SQ + 127) / 128), narrow = (u64)s.B * s.HK * ((R + 15) / 16);
-    // Split or not, in steps of a workgroup on 64 keys (1.2 us at 128 dims in 16 bits).  Rows are worth a workgroup each 64 queries if
-    // its chain of steps is shorter than the rows' shares of the chip: a split step of 16 rows and 32 keys costs a wave 2.25 of
-    // them, several waves at a time in each SIMD, and joining shares costs 6.  bf16, 32 heads on 8, 128 dims, queries x keys:
-    // 128 x 8192 92 us split, 181 not; 40 x 32768 115 and 707; 8 heads of 512 x 512 20.9 and 15.8, 256 x 256 7.2 and 10.1.
-    // Up to 32 rows per key head, a single token among them, are split in any case.
+    // Split or not, by the time either takes (SplitOrNot): rows are worth a workgroup each 64 queries if its chain of steps is shorter
+    // than the rows' shares of the chip.  Up to 32 rows per key head, a single token among them, are split in any case.
     constexpr int most = most_waves<T, DP>();
     constexpr u64 resident = 163840 / SplitLds<T, DP, 4>::kBytes < 4 ? 163840 / SplitLds<T, DP, 4>::kBytes : 4;
     // what a row can see at most: the whole cache, or the window and the leading keys
@@ -627,10 +641,12 @@ template <class T, int DP> int forward(aixk_ctx* ctx, const Call& c)
     };
     const u64 keys = reach(std::min<u64>((u64)(u32)s.SQ, 16));
     const bool one = most > 4 && narrow < (u64)ctx->cus && keys > 4 * kSplitKeys && keys <= 3u * most * kSplitKeys;
-    const double block_steps = (double)((reach(64) + 63) / 64), split_steps = (double)((keys + kSplitKeys - 1) / kSplitKeys);
-    const double split_cost = one ? 2.25 * (double)(((u64)split_steps + most - 1) / most)
-                                  : 6.0 + 2.25 * (double)narrow * split_steps / (double)((u64)ctx->cus * 4 * std::min<u64>(resident, 2));
-    if (R > 32 && (split_cost >= block_steps || R >= (1ull << 31))) {
+    typedef SplitOrNot<sizeof(T), DP> Us;
+    const u64 split_steps = (keys + kSplitKeys - 1) / kSplitKeys;
+    const double block_cost = Us::block + Us::block_step * (double)((reach(64) + 63) / 64);
+    const double split_cost = one ? 4.5 + Us::split_step * (double)((split_steps + most - 1) / most)
+                                  : Us::split + Us::split_step * (double)narrow * (double)split_steps / (double)((u64)ctx->cus * 4 * std::min<u64>(resident, 2));
+    if (R > 32 && (split_cost >= block_cost || R >= (1ull << 31))) {
         // 32 queries to a wave where that leaves a workgroup for every compute unit, and above 128 head dims, where 16 queries to a
         // wave read too much LDS for what they multiply (8 heads of 1000 x 192, few workgroups: 25.3 us against 36.0); f32 and
         // small grids: 16 queries to a wave.
