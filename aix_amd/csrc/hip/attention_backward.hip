@@ -474,11 +474,12 @@ template <class T, int DP> int backward(aixk_ctx* ctx, const Call& c, BackwardAr
     constexpr u64 resident = KeyBlock<T, DP>::kWaves * 256 / KeyBlock<T, DP>::kThreads;
     const u64 slots = (u64)ctx->cus * resident;
     const u64 seen = s.window && (u64)s.window + keys < (u64)(u32)s.SQ ? (u64)s.window + keys : (u64)(u32)s.SQ;      // queries of a tile at most
-    const u64 steps = ((u64)s.G * seen + KeyBlock<T, DP>::kRows - 1) / KeyBlock<T, DP>::kRows, more = seen ? std::min<u64>(((u32)s.SQ + seen - 1) / seen, 32) : 1;
+    const u64 steps = ((u64)s.G * seen + KeyBlock<T, DP>::kRows - 1) / KeyBlock<T, DP>::kRows;
     if (s.window && s.sinks && seen) {
         a.lead = ((u32)s.sinks + keys - 1) / keys;
         if (a.lead > a.tiles) a.lead = a.tiles;
     }
+    const u64 more = a.lead ? std::min<u64>(((u32)s.SQ + seen - 1) / seen, 32) : 1;      // shares of a tile with leading keys for each of another's, at most
     // keys with shares of their own: whole tiles if the other tiles have shares too, else the leading keys
     auto lead_keys = [&](u64 sp) { return a.lead ? std::min<u64>(sp > 1 ? (u64)a.lead * keys : (u64)(u32)s.sinks, (u64)(u32)s.SK) : 0; };
     struct Plan { u64 splits, more, planes, grid; };
@@ -489,7 +490,7 @@ template <class T, int DP> int backward(aixk_ctx* ctx, const Call& c, BackwardAr
         Plan best{};
         double least = -1.0;
         for (u64 sp = 1; sp <= 64 && (sp == 1 || sp * 4 <= steps); ++sp)
-            for (u64 mo = a.lead ? more : 1;; mo = (mo + 1) / 2) {
+            for (u64 mo = more;; mo = (mo + 1) / 2) {
                 const u64 n = heads * (a.lead * sp * mo + (a.tiles - a.lead) * sp);
                 const u64 shares = (sp > 1 ? sp * rows : 0) + (sp * mo > 1 ? (sp > 1 ? sp * (mo - 1) : mo) * heads * lead_keys(sp) : 0);
                 // steps of a workgroup, and of one on leading keys: all queries of theirs over its shares, or (one share for the
