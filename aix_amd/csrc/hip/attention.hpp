@@ -211,7 +211,9 @@ template <class T> __device__ __forceinline__ typename Mma<T>::Frag load8(const 
 
 // Elements from d on lie past the head dim and their products are left out: f32, whose matrix instructions take 16 times as
 // long as the branch does, and head dims above 128, where the branches also keep the compiler from holding every operand of a
-// loop at once (attention_dkdv_k at 256: 263 spilled registers, 16 with them).  The other kernels multiply the zeros and stay free of branches.
+// loop at once (attention_dkdv_k at 256: 263 spilled registers, 16 with them).  There they have a price: loops that end at
+// such a branch stay rolled, and the register arrays they index become private memory (bytes per lane at 256 dims: attention_split_k 272 in
+// 16 bits; attention_dq_k 528, f32 1040; attention_dkdv_k 336, f16 384, f32 1104).  The other kernels multiply the zeros and stay free of branches.
 template <class T, int DP> __device__ __forceinline__ bool past(int d, u32 DW) { return (sizeof(T) == 4 || DP > 128) && d >= (int)DW; }
 
 // Waves per SIMD a kernel is compiled for: two where a wave's share of the 512 registers then holds its accumulators, fragments

@@ -2368,6 +2368,8 @@ int matmul_mfma(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, c
 // What would be left to its LDS-tiled kernel -- contractions without whole 16-byte words (the rows of a batch in a weight
 // gradient), results below 64 x 64 elements -- has its operands copied K-contiguous with zeros up to a whole word.
 // (f32, the backward pass of [11127, 1216] x [1216, 128]: 2334 -> 130 us; [1, 2624] x [2624, 64]: 347 -> 15 us.)
+// f32 operands that the LDS-tiled kernel would multiply in f32 may so go through three bf16 planes each (gemm_x3_k: six products of
+// planes, off by 2^-22 of a term, sums in f32): the choice aixk_matmul makes for its larger shapes, made here for all.
 int matmul_plain(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_tensor* b, const aixhip_tensor* out)
 {
     const uint64_t M = a->shape[0], K = a->shape[1], N = b->shape[1];

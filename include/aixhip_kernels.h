@@ -241,8 +241,9 @@ int32_t aixk_matmul_grouped(aixk_ctx* ctx, const aixhip_tensor* a, const aixhip_
  *   0 <= p,  j < lengths[b],  (causal: j <= p),  (window > 0: |p - j| < window, or j < sinks).
  * lengths NULL: every key; starts NULL: the queries are the last ones, starts[b] = lengths[b] - queries.  Both are int32
  * [batch] in device memory, read when the kernels run (a captured call follows their current values); lengths beyond the
- * keys count as all of them, negative ones as none; starts are taken within +- 2^29.  Keys at and behind a length are never
- * read.  A query that sees no key gives zeros and lse = -infinity, and no gradient.  Unseen pairs in
+ * keys count as all of them, negative ones as none; starts are taken within +- 2^29.  What keys and values hold at and behind a
+ * length does not matter (it is read only where whole operands are copied: head dims or strides without 16-byte rows).  A query that
+ * sees no key, or only scores of -infinity, gives zeros and lse = -infinity, and no gradient.  Unseen pairs in
  * front of a length take part in the products with a weight of zero: keys and values there, queries and their gradients must be
  * finite (their scores need not be). */
 typedef struct aixk_attention_spec {
@@ -291,7 +292,9 @@ int32_t aixk_rotary(aixk_ctx* ctx, const aixhip_tensor* q, const aixhip_tensor* 
 /* A matrix product with what usually follows it: z = a . b + bias, out = act(z) + residual.  a [M, K] and b [K, N] are any 2-D
  * views of one element type, bias [N] or [1, N], residual [M, N] any view (a broadcast one too); out and pre are dense [M, N].
  * pre, if given, receives z rounded to the element type (what the backward pass needs); the activation is taken of z itself.
- * out may be the residual itself (the same dense view).  GELU is the tanh form, 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))). */
+ * out may be the residual itself (the same dense view).  16-bit products finish in the kernel that forms them; f32 products are formed
+ * first and finished in a pass of their own, and their operands may go through the matrix unit as three bf16 planes each, which is
+ * 2^-22 of a product's terms where an f32 sum rounds each to 2^-24 (as in aixk_matmul, here for every shape).  GELU is the tanh form, 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))). */
 enum aixk_activation { AIXK_ACT_NONE = 0, AIXK_ACT_RELU = 1, AIXK_ACT_GELU = 2, AIXK_ACT_SILU = 3 };
 typedef struct aixk_epilogue {
     const aixhip_tensor* bias;       /* or NULL */
